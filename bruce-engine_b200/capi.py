@@ -33,8 +33,14 @@ class CPages(C.Structure):
                 ("n_pages", C.c_int), ("n_tables", C.c_int), ("max_pages", C.c_int), ("page_len", C.c_int)]
 
 
+class CSinks(C.Structure):
+    """battn_sinks: how many first positions stay visible beside a window, and the buffers that keep them for a ring."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_sink", C.c_int), ("cap", C.c_int)]
+
+
 _P, _I, _SZP = C.c_void_p, C.c_int, C.POINTER(C.c_size_t)
 _PG = C.POINTER(CPages)
+_SK = C.POINTER(CSinks)
 
 # name -> (restype, argtypes); exactly the symbols include/battn.h declares
 SIGNATURES = {
@@ -71,6 +77,10 @@ SIGNATURES = {
     "battn_verify_paged": (_I, [_P, _P, _P, _PG] + [_P] * 4 + [_I, _I, _P]),
     "battn_prefill_paged": (_I, [_P, _P, _P, _PG, _I, _P, _P, _I, _P]),
     "battn_attend_exact_paged": (_I, [_P, _P, _P, _PG] + [_P] * 4 + [_I, _I, _I, _P]),
+    "battn_sinks_bytes": (_I, [_P, _I, _SZP]),
+    "battn_sinks_store": (_I, [_P, _P, _P, _SK] + [_P] * 3 + [_I, _I, _P]),
+    "battn_attend_sinks": (_I, [_P] * 5 + [_SK] + [_P] * 4 + [_I, _I, _I, _P]),
+    "battn_attend_sinks_paged": (_I, [_P] * 3 + [_PG, _SK] + [_P] * 4 + [_I, _I, _P]),
     "battn_xchg_create": (_I, [_P, _I, _I, _I, C.POINTER(_P), _P]),
     "battn_xchg_connect": (_I, [_P, _P]),
     "battn_xchg_area": (_I, [_P, C.POINTER(_P), _SZP]),

@@ -14,6 +14,7 @@
 #include "qkv_prep.cuh"
 #include "prefill.cuh"
 #include "prefill_hd128.cuh"
+#include "sinks.cuh"
 #include "verify.cuh"
 #include "verify_tc.cuh"
 
@@ -53,6 +54,11 @@ inline int cuda_fail(battn_handle* h, cudaError_t e) {
 
 inline int nt_index(int RG) { return RG <= 8 ? 0 : (RG <= 16 ? 1 : 2); }
 
+template <typename Params>
+cudaError_t allow_smem(void (*kernel)(const Params), size_t bytes) {
+    return cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
 template <int HD, int NT>
 cudaError_t fd_prepare(battn_handle* h, int idx) {
     auto kern = fd::k_flash_decode<HD, NT>;
@@ -84,9 +90,16 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     cudaError_t e;
     if ((e = vw_prepare<HD>(h)) != cudaSuccess) return e;
     if (HD == 128) {
-        e = cudaFuncSetAttribute((const void*)vt::k_verify_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX);
-        if (e != cudaSuccess) return e;
+        if ((e = allow_smem(vt::k_verify_tc<VAR_PLAIN>, SMEM_MAX)) != cudaSuccess) return e;
+        if ((e = allow_smem(vt::k_verify_tc<VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
+        if ((e = allow_smem(pf128::k_prefill_hd128<false, VAR_SINK>, pf128::TOTAL)) != cudaSuccess) return e;
+        if ((e = allow_smem(pf128::k_prefill_hd128<true, VAR_SINK>, pf128::TOTAL_PAIR)) != cudaSuccess) return e;
+    } else {
+        if ((e = allow_smem(pf::k_prefill<256, 64, VAR_SINK>, pf::Cfg<256, 64>::TOTAL)) != cudaSuccess) return e;
     }
+    if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
+    if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
+    if ((e = allow_smem(fd::k_flash_decode<HD, 2, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if (HD == 128) {
         e = cudaFuncSetAttribute((const void*)pf128::k_prefill_hd128<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, pf128::TOTAL);
         if (e == cudaSuccess)
@@ -169,6 +182,15 @@ cudaError_t launch_pdl(void (*kernel)(const Params), dim3 grid, dim3 block, size
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+// makes the handle's device current for the launches of one call, whatever device the caller's thread had
+struct DeviceScope {
+    int prev = -1, dev;
+    explicit DeviceScope(int d) : dev(d) {
+        if (cudaGetDevice(&prev) == cudaSuccess && prev != dev) cudaSetDevice(dev);
+    }
+    ~DeviceScope() { if (prev >= 0 && prev != dev) cudaSetDevice(prev); }
+};
+
 // event pair around the main kernel of a call while profiling is on
 struct ProfScope {
     battn_handle* h; cudaStream_t st; int idx;
@@ -246,7 +268,8 @@ struct PrologueIn {
 };
 
 template <int HD, int NT>
-cudaError_t launch_fd_kernel(const fd::Params& P, int grid, size_t smem, cudaStream_t st) {
+cudaError_t launch_fd_kernel(const fd::Params& P, int grid, size_t smem, cudaStream_t st, int var) {
+    if (var == VAR_SINK) return launch_pdl(fd::k_flash_decode<HD, NT, 0, VAR_SINK>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
     if constexpr (NT == 1) {
         if (P.q_raw) return launch_pdl(fd::k_flash_decode<HD, 1, 2>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
         if (P.k_new) return launch_pdl(fd::k_flash_decode<HD, 1, 1>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
@@ -259,8 +282,9 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
                  const int* pos, const int* kslot, const int* act, void* ws, int n_seq, int rows, int is_swa,
                  cudaStream_t st, const XchgView* xv = nullptr, int* epoch_ptr = nullptr, int epoch_advance = 0,
                  const PagedView* pv = nullptr, const float* k_new = nullptr, const float* v_new = nullptr,
-                 const PrologueIn* pro = nullptr) {
+                 const PrologueIn* pro = nullptr, const SinkView* sink = nullptr) {
     const Geom& g = h->g;
+    const int var = sink ? VAR_SINK : VAR_PLAIN;
     const int RG = rows * g.G;
     if (RG > 32) return BATTN_ERR_CAPACITY;
     const int idx = nt_index(RG);
@@ -275,6 +299,7 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
     P.epoch_ptr = epoch_ptr; P.epoch_advance = epoch_advance;
     P.cph = 0;
+    if (sink) P.sink = *sink;
     P.q_raw = pro ? pro->q_raw : nullptr; P.sqk = pro ? pro->sqk : nullptr; P.cs = pro ? pro->cs : nullptr;
     P.sn = pro ? pro->sn : nullptr; P.table_off = pro ? pro->table_off : 0;
     P.k_new = k_new; P.v_new = v_new; P.kvk_w = const_cast<uint8_t*>(kvk); P.kvv_w = const_cast<uint8_t*>(kvv);
@@ -294,7 +319,8 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
         // ring, hence the window bound; very large batches exceed its shared memory and take the kernel below)
         if (n_seq == 1 && h->num_sms >= g.Hkv) P.cph = h->num_sms / g.Hkv;
         ProfScope prof(h, st);
-        e = launch_pdl(vt::k_verify_tc, dim3(h->num_sms), dim3(vt::NTHREADS), vt::smem_bytes(n_seq), st, P);
+        e = launch_pdl(sink ? vt::k_verify_tc<VAR_SINK> : vt::k_verify_tc<VAR_PLAIN>, dim3(h->num_sms), dim3(vt::NTHREADS),
+                       vt::smem_bytes(n_seq), st, P);
     } else if (RG > 16) {
         // 5..8 rows: the wide verify kernel (each warp owns 8 pairs over all keys of a tile)
         const size_t smem = g.HD == 128 ? vw::smem_bytes<128>(n_seq) : vw::smem_bytes<256>(n_seq);
@@ -305,8 +331,9 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
         const int grid = h->num_sms * per_sm;
         if (n_seq == 1 && grid >= g.Hkv) P.cph = grid / g.Hkv;
         ProfScope prof(h, st);
-        e = g.HD == 128 ? launch_pdl(vw::k_verify_wide<128>, dim3(grid), dim3(vw::NTHREADS), smem, st, P)
-                        : launch_pdl(vw::k_verify_wide<256>, dim3(grid), dim3(vw::NTHREADS), smem, st, P);
+        e = launch_pdl(g.HD == 128 ? (sink ? vw::k_verify_wide<128, VAR_SINK> : vw::k_verify_wide<128>)
+                                   : (sink ? vw::k_verify_wide<256, VAR_SINK> : vw::k_verify_wide<256>),
+                       dim3(grid), dim3(vw::NTHREADS), smem, st, P);
     } else {
         size_t smem;
         if (g.HD == 128) smem = idx == 0 ? fd::smem_bytes<128, 1>(RG, n_seq) : fd::smem_bytes<128, 2>(RG, n_seq);
@@ -319,8 +346,8 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
         fd_grid = grid;
         if (n_seq == 1 && grid >= g.Hkv) P.cph = grid / g.Hkv;     // one sequence: no share crosses a kv head
         ProfScope prof(h, st);
-        if (g.HD == 128) e = idx == 0 ? launch_fd_kernel<128, 1>(P, grid, smem, st) : launch_fd_kernel<128, 2>(P, grid, smem, st);
-        else             e = idx == 0 ? launch_fd_kernel<256, 1>(P, grid, smem, st) : launch_fd_kernel<256, 2>(P, grid, smem, st);
+        if (g.HD == 128) e = idx == 0 ? launch_fd_kernel<128, 1>(P, grid, smem, st, var) : launch_fd_kernel<128, 2>(P, grid, smem, st, var);
+        else             e = idx == 0 ? launch_fd_kernel<256, 1>(P, grid, smem, st, var) : launch_fd_kernel<256, 2>(P, grid, smem, st, var);
     }
     if (e != cudaSuccess) return cuda_fail(h, e);
     MergeParams M{};
@@ -328,7 +355,7 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     M.n_rows = n_seq * rows; M.rows = rows; M.Hq = g.Hq; M.Hkv = g.Hkv; M.G = g.G;
     M.count = 0; M.log2_domain = 1; M.out_f16 = g.out_f16; M.hdr = P.hdr; M.status = h->d_status;
     M.cph = P.cph;
-    if (P.early && fd_grid > 0 && n_seq == 1) {
+    if (P.early && fd_grid > 0 && n_seq == 1 && var == VAR_PLAIN) {
         // the merge recomputes the cut from the positions while it waits for the decode kernel
         M.pre_grid = fd_grid; M.pre_tile = fd::TILE;
         M.pos = pos; M.kslot = kslot; M.act = act; M.is_swa = is_swa; M.W = g.W; M.slot_ctx = P.slot_ctx; M.n_slots = P.n_slots;
@@ -341,10 +368,18 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     return e == cudaSuccess ? BATTN_OK : cuda_fail(h, e);
 }
 
+// what a variant of the prompt call adds: the device-resident slot and activity of its sequence, and its own inputs
+struct ChunkVariant {
+    int var;
+    const int* kslot;
+    const int* act;
+    SinkView sink;               // VAR_SINK
+};
+
 // prompt chunk on the tcgen05 kernel: one CTA per (128-row M tile, kv head), normalised output
 int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk, const uint8_t* kvv, const int* pos,
                    void* ws, int rows, int is_swa, cudaStream_t st, const GateNormParams* gn = nullptr,
-                   const PagedView* pv = nullptr, int table_row = 0) {
+                   const PagedView* pv = nullptr, int table_row = 0, const ChunkVariant* cv = nullptr) {
     const Geom& g = h->g;
     if (128 % g.G) return BATTN_ERR_ARG;
     pf::Params P;
@@ -355,13 +390,17 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
     P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
     apply_paging(P, pv);
     if (pv) P.slot = table_row;
+    const int var = cv ? cv->var : VAR_PLAIN;
+    if (cv) {
+        P.kslot = cv->kslot; P.act = cv->act; P.n_slots = pv ? pv->n_tables : g.n_slots; P.sink = cv->sink;
+    }
     // early KV streaming: only behind the append / prologue of exactly this chunk, or no cache write
     P.early = h->early_stream &&
               (h->kvw_kind == 0 || (h->kvw_kind == 1 && h->kvw_pos == pos && h->kvw_nseq == 1 && h->kvw_rows == rows) ||
                (h->kvw_kind == 3 && h->kvw_cache != (const void*)kvk));
     h->kvw_kind = 0;
     const int MR = 128 / g.G;
-    P.nsplit = prefill_splits(h, rows, is_swa);
+    P.nsplit = prefill_splits(h, rows, is_swa || var == VAR_SINK);
     P.recs = (P.nsplit > 1 || gn) ? reinterpret_cast<float*>(ws) : nullptr;
     const dim3 grid((rows + MR - 1) / MR, g.Hkv, P.nsplit);
     {
@@ -377,11 +416,11 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
             attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
             attr[1].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr; cfg.numAttrs = 2;
-            cudaLaunchKernelEx(&cfg, pf128::k_prefill_hd128<true>, P);
+            cudaLaunchKernelEx(&cfg, var == VAR_SINK ? pf128::k_prefill_hd128<true, VAR_SINK> : pf128::k_prefill_hd128<true>, P);
         } else if (g.HD == 128) {
-            launch_pdl(pf128::k_prefill_hd128<false>, grid, dim3(pf128::NTHREADS), pf128::TOTAL, st, P);
+            launch_pdl(var == VAR_SINK ? pf128::k_prefill_hd128<false, VAR_SINK> : pf128::k_prefill_hd128<false>, grid, dim3(pf128::NTHREADS), pf128::TOTAL, st, P);
         }
-        else             launch_pdl(pf::k_prefill<256, 64>, grid, dim3(pf::NTHREADS), pf::Cfg<256, 64>::TOTAL, st, P);
+        else             launch_pdl(var == VAR_SINK ? pf::k_prefill<256, 64, VAR_SINK> : pf::k_prefill<256, 64>, grid, dim3(pf::NTHREADS), pf::Cfg<256, 64>::TOTAL, st, P);
     }
     h->launches += 1;
     cudaError_t e = cudaGetLastError();
@@ -400,6 +439,10 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
         M.mode = MERGE_GATHERED; M.part = P.recs; M.out = out; M.rec_out = nullptr;
         M.n_rows = rows; M.rows = 1; M.Hq = g.Hq; M.Hkv = g.Hkv; M.G = g.G;
         M.count = P.nsplit; M.log2_domain = 1; M.out_f16 = g.out_f16; M.status = h->d_status;
+        if (cv) {                                // an idle sequence left no records
+            M.pos = pos; M.kslot = cv->kslot; M.act = cv->act; M.is_swa = is_swa; M.W = g.W; M.slot_ctx = P.slot_ctx;
+            M.n_slots = P.n_slots;
+        }
         // (head_dim 128: programmatic launch, the merge's blocks are resident and past their launch when the prompt
         // kernel drains -- 2 us less on a short chunk; at head_dim 256, where every 512-row chunk is split and the merge
         // has thousands of blocks, the early launch cost 2 % and the plain launch stays)
@@ -870,6 +913,81 @@ int battn_attend_exact_paged(battn_handle* h, void* out, const void* q, const ba
     if (!ws || ((uintptr_t)ws & 15) || nsplit < 1 || nsplit > MAX_SPLITS) return BATTN_ERR_ARG;
     return launch_exact(h, out, nullptr, q, pages->pool_k, pages->pool_v, pos, ktab, act, ws, n_seq, rows_per_seq, nsplit,
                         0, (cudaStream_t)stream, &pv);
+}
+
+// ---- sliding window with sinks ------------------------------------------------------------------------------
+int battn_sinks_bytes(const battn_handle* h, int cap, size_t* out_bytes) {
+    if (!h || !out_bytes || cap < SINK_TILE || cap % SINK_TILE) return BATTN_ERR_ARG;
+    *out_bytes = (size_t)h->g.n_slots * h->g.Hkv * cap * h->g.rec;
+    return BATTN_OK;
+}
+
+// a caller's sinks, validated: buffers beside a ring, none for a cache that keeps its first positions
+static int sink_view(const Geom& g, const battn_sinks* sinks, int ring, SinkView& v) {
+    if (!sinks || sinks->n_sink < 0 || sinks->n_sink > g.W) return BATTN_ERR_ARG;
+    if (ring) {
+        if (!sinks->k || !sinks->v || (((uintptr_t)sinks->k | (uintptr_t)sinks->v) & 15)) return BATTN_ERR_ARG;
+        if (sinks->cap < SINK_TILE || sinks->cap % SINK_TILE || sinks->cap < sinks->n_sink) return BATTN_ERR_ARG;
+        v.k = sinks->k; v.v = sinks->v; v.cap = sinks->cap;
+    } else if (sinks->k || sinks->v) {
+        return BATTN_ERR_ARG;
+    }
+    v.n = sinks->n_sink;
+    return BATTN_OK;
+}
+
+int battn_sinks_store(battn_handle* h, const uint8_t* kvk, const uint8_t* kvv, const battn_sinks* sinks, const int* pos,
+                      const int* kslot, const int* act, int n_seq, int rows_per_seq, void* stream) {
+    int rc = check_seq_args(h, kvk, kvv, kvk, kvv, pos, kslot, n_seq, rows_per_seq, MAX_PREFILL);
+    if (rc) return rc;
+    const Geom& g = h->g;
+    SinkView v;
+    if ((rc = sink_view(g, sinks, 1, v))) return rc;
+    if (rows_per_seq > g.ring) return BATTN_ERR_CAPACITY;
+    const DeviceScope dev(h->device);
+    SinkStoreParams P;
+    P.kvk = kvk; P.kvv = kvv; P.sk = sinks->k; P.sv = sinks->v; P.pos = pos; P.kslot = kslot; P.act = act;
+    P.rows = rows_per_seq; P.Hkv = g.Hkv; P.rec = g.rec; P.ring = g.ring; P.cap = v.cap; P.n_slots = g.n_slots;
+    P.status = h->d_status;
+    h->kvw_kind = 2;                     // sink tiles are cache rows: no call streams early behind this one
+    cudaError_t e = launch_pdl(k_sinks_store, dim3(n_seq, g.Hkv, 2), dim3(256), 0, (cudaStream_t)stream, P);
+    h->launches += 1;
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? BATTN_OK : cuda_fail(h, e);
+}
+
+static int attend_sinks_impl(battn_handle* h, void* out, const void* q, const uint8_t* kvk, const uint8_t* kvv,
+                             const battn_sinks* sinks, const int* pos, const int* kslot, const int* act, void* ws, int rows,
+                             int n_seq, int is_swa, void* stream, const PagedView* pv) {
+    int rc = check_seq_args(h, out, q, kvk, kvv, pos, kslot, n_seq, rows, MAX_PREFILL);
+    if (rc) return rc;
+    if (!ws || ((uintptr_t)ws & 15)) return BATTN_ERR_ARG;
+    const Geom& g = h->g;
+    ChunkVariant cv{VAR_SINK, kslot, act, {}};
+    if ((rc = sink_view(g, sinks, is_swa, cv.sink))) return rc;
+    const DeviceScope dev(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rows <= MAX_VERIFY && rows * g.G <= 32)
+        return launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, rows, is_swa, st, nullptr, nullptr, 0, pv,
+                            nullptr, nullptr, nullptr, &cv.sink);
+    // a prompt chunk: one sequence, and the bounds of battn_prefill
+    if (n_seq != 1 || (is_swa && rows > g.W)) return BATTN_ERR_CAPACITY;
+    if (g.W < 64) return BATTN_ERR_ARG;
+    return launch_prefill(h, out, q, kvk, kvv, pos, ws, rows, is_swa, st, nullptr, pv, 0, &cv);
+}
+
+int battn_attend_sinks(battn_handle* h, void* out, const void* q, const uint8_t* kvk, const uint8_t* kvv,
+                       const battn_sinks* sinks, const int* pos, const int* kslot, const int* act, void* ws, int rows,
+                       int n_seq, int is_swa, void* stream) {
+    return attend_sinks_impl(h, out, q, kvk, kvv, sinks, pos, kslot, act, ws, rows, n_seq, is_swa != 0, stream, nullptr);
+}
+
+int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const battn_pages* pages, const battn_sinks* sinks,
+                             const int* pos, const int* ktab, const int* act, void* ws, int rows, int n_seq, void* stream) {
+    PagedView pv;
+    const int rc = paged_view(pages, pv);
+    if (rc) return rc;
+    return attend_sinks_impl(h, out, q, pages->pool_k, pages->pool_v, sinks, pos, ktab, act, ws, rows, n_seq, 0, stream, &pv);
 }
 
 int battn_xchg_create(battn_handle* h, int rank, int world, int max_rows, battn_xchg** out_x, void* ipc_handle_out) {

@@ -235,4 +235,50 @@ __device__ __forceinline__ SeqRange seq_range(const int* __restrict__ pos, const
     return s;
 }
 
+// ---- sliding window with sinks ---------------------------------------------------------------------
+// Attention with sinks: a row at position p sees the keys of its window (p - W, p] and the first n positions of its
+// sequence.  The visible key tiles of a sequence are the sink tiles [0, ceil(n / TILE)) below the window and the
+// window's tiles, walked in that order; a sink tile that the window has not passed yet is a window tile and counts once.
+// k, v: buffers [slot][kv head][cap positions][record] that hold the first `cap` positions (whole tiles) of every
+// sequence of a ring layer, where the ring has replaced them; every tile below cap is read from them, those of a young
+// sequence too.  k == nullptr: a cache that still holds its first positions, read in place.
+constexpr int SINK_TILE = 128;              // cap is a multiple of the widest key tile
+struct SinkView {
+    const uint8_t* k = nullptr;
+    const uint8_t* v = nullptr;
+    int n = 0, cap = 0;
+};
+// which work the attention kernels do besides the plain call (template parameter VAR)
+enum { VAR_PLAIN = 0, VAR_SINK = 1, VAR_TRACK = 2 };
+
+// seq_range with the window applied whatever the layer's storage (a cache read in place is not a ring)
+template <int VAR>
+__device__ __forceinline__ SeqRange seq_keys(const int* __restrict__ pos, const int* __restrict__ kslot,
+                                             const int* __restrict__ act, int i, int rows, int is_swa, int W, int slot_ctx,
+                                             int n_slots, int* status) {
+    SeqRange s = seq_range(pos, kslot, act, i, rows, is_swa, W, slot_ctx, n_slots, status);
+    if (VAR == VAR_SINK && s.active) s.lo = max(0, s.p0 + 1 - W);
+    return s;
+}
+
+// the key tiles of a sequence whose rows see [lo, hi) and, with sinks, the first n positions: tile number at(u), u < count
+template <int VAR, int TILE>
+struct KeyTiles {
+    int first, ns;
+    __device__ __forceinline__ KeyTiles(int lo, const SinkView& sk)
+        : first(lo / TILE), ns(VAR == VAR_SINK ? min((sk.n + TILE - 1) / TILE, first) : 0) {}
+    __device__ __forceinline__ int count(int hi) const { return (hi + TILE - 1) / TILE - first + ns; }
+    __device__ __forceinline__ int at(int u) const { return VAR == VAR_SINK && u < ns ? u : first - ns + u; }
+};
+// is `key` hidden from a row whose window starts at `low`?
+template <int VAR>
+__device__ __forceinline__ bool below_window(int key, int low, const SinkView& sk) {
+    return key < low && !(VAR == VAR_SINK && key < sk.n);
+}
+// does every row see all keys of [t0, t0 + TILE), as far as the window goes?
+template <int VAR, int TILE>
+__device__ __forceinline__ bool tile_in_window(int t0, int full_lo, const SinkView& sk) {
+    return t0 >= full_lo || (VAR == VAR_SINK && t0 + TILE <= sk.n);
+}
+
 }  // namespace battn

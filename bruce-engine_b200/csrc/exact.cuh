@@ -204,7 +204,7 @@ struct MergeParams {
     int count;             // REGULAR: splits; GATHERED: parts
     int log2_domain;       // records carry m in log2 units (flash-decode partials)
     int out_f16;
-    // REGULAR only: skip rows of inactive sequences
+    // REGULAR, and GATHERED behind a prompt chunk that may be idle (else null): skip rows of inactive sequences
     const int* pos; const int* kslot; const int* act;
     int is_swa, W, slot_ctx, n_slots;
     int* status;
@@ -246,6 +246,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_merge(const MergeParams P) {
         base = P.part + (((size_t)rowidx * P.Hkv + kvh) * count * P.G + h) * (size_t)(HD + 2);
         stride = (size_t)P.G * (HD + 2);
     } else {                                     // MERGE_GATHERED
+        if (P.pos) {                             // the records of one prompt chunk, absent when its sequence was skipped
+            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.n_rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+            if (!sr.active) return;
+        }
         count = P.count;
         base = P.part + ((size_t)rowidx * P.Hq + hq) * (size_t)(HD + 2);
         stride = (size_t)P.n_rows * P.Hq * (HD + 2);

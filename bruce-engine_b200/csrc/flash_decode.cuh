@@ -83,6 +83,7 @@ struct Params {
     const float* v_new;
     uint8_t* kvk_w;  // the caches again, writable
     uint8_t* kvv_w;
+    SinkView sink;   // VAR_SINK
 };
 
 template <int HD>
@@ -105,7 +106,8 @@ __device__ __forceinline__ int perm16(int kappa) { return kappa ^ ((kappa >> 2) 
 
 // AP: 1 = the decode call that appends its own (prepared) row, 2 = the one that also runs the QKV prologue of its row
 // (separate instances, so that the plain kernel carries none of it)
-template <int HD, int NT, int AP = 0>
+// VAR: VAR_SINK = sliding window with sinks
+template <int HD, int NT, int AP = 0, int VAR = VAR_PLAIN>
 __global__ void __launch_bounds__(NTHREADS, (NT == 1 ? 3 : (NT == 2 ? 2 : 1)))
 k_flash_decode(const Params P) {
     using C = Cfg<HD>;
@@ -137,15 +139,15 @@ k_flash_decode(const Params P) {
     if (P.n_seq == 1) {
         // one sequence (decode / verify of a single stream): no prefix sum, one barrier
         if (tid == 0) {
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, 0, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
             cum[0] = 0;
-            cum[1] = sr.active ? ((sr.hi + TILE - 1) / TILE - sr.lo / TILE) : 0;
+            cum[1] = sr.active ? KeyTiles<VAR, TILE>(sr.lo, P.sink).count(sr.hi) : 0;
         }
         __syncthreads();
     } else {
         for (int i = tid; i < P.n_seq; i += NTHREADS) {
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
-            cum[i + 1] = sr.active ? ((sr.hi + TILE - 1) / TILE - sr.lo / TILE) : 0;
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+            cum[i + 1] = sr.active ? KeyTiles<VAR, TILE>(sr.lo, P.sink).count(sr.hi) : 0;
         }
         if (tid == 0) cum[0] = 0;
         __syncthreads();
@@ -186,23 +188,23 @@ k_flash_decode(const Params P) {
             bool waited = !early || blockIdx.x == 0;
             for (int g = g0; g < g1;) {
                 const Piece pc = locate(g, g1, cum, P.n_seq, P.Hkv);
-                const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
+                const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
                                               P.n_slots, P.status);
                 const size_t hb = ((size_t)sr.slot * P.Hkv + pc.kvh) * P.pstride * (size_t)REC;
-                const int tile0 = sr.lo / TILE + pc.tl;
+                const KeyTiles<VAR, TILE> kt(sr.lo, P.sink);
                 // paged cache: the table entry of the next tile is fetched one tile ahead, so the look-up never sits
                 // between a freed stage and its refill
                 const int* trow = P.pg.table ? P.pg.table + (size_t)sr.slot * P.pg.max_pages : nullptr;
-                int page_nx = trow ? trow[(tile0 * TILE) >> P.pg.shift] : 0;
+                int page_nx = trow ? trow[(kt.at(pc.tl) * TILE) >> P.pg.shift] : 0;
                 for (int t = 0; t < pc.n; ++t, ++cnt) {
                     const int s = cnt % STAGES, use = cnt / STAGES;
-                    const int page = page_nx;
-                    if (trow && t + 1 < pc.n) page_nx = trow[((tile0 + t + 1) * TILE) >> P.pg.shift];
+                    const int page = page_nx, tile = kt.at(pc.tl + t);
+                    if (trow && t + 1 < pc.n) page_nx = trow[(kt.at(pc.tl + t + 1) * TILE) >> P.pg.shift];
                     // early streaming stops at the tile that holds the row BEFORE this step's own rows (the decode
                     // kernel of a preceding appending call, which writes that row, may still be running: its merge
                     // releases this launch before it waits), and before the first stage that needs the consumers
                     // (they do not start before the predecessor has finished)
-                    if (!waited && ((tile0 + t + 1) * TILE >= sr.p0 || use > 0)) {
+                    if (!waited && ((tile + 1) * TILE >= sr.p0 || use > 0)) {
                         pdl_wait();
                         pdl_trigger();
                         waited = true;
@@ -214,15 +216,17 @@ k_flash_decode(const Params P) {
                         }
                     }
                     if (*(volatile int*)&s_abort) continue;     // stop issuing; consumers skip their waits
-                    const int sp = ((tile0 + t) * TILE) & P.ring_mask;
-                    const int nk = trow ? TILE : min(TILE, P.pstride - sp);
+                    const int sp = (tile * TILE) & P.ring_mask;
+                    const bool kept = VAR == VAR_SINK && P.sink.k && tile * TILE < P.sink.cap;   // from the sink buffers
+                    const int nk = trow || kept ? TILE : min(TILE, P.pstride - sp);
                     const uint32_t bytes = (uint32_t)nk * REC;
                     const size_t src = trow ? kv_rec_index_page(P.pg, page, pc.kvh, P.Hkv, sp, P.status) * (size_t)REC
+                                     : kept ? (((size_t)sr.slot * P.Hkv + pc.kvh) * P.sink.cap + tile * TILE) * (size_t)REC
                                             : hb + (size_t)sp * REC;
                     uint8_t* dstk = stages + (size_t)s * 2 * TILE_BYTES;
                     mbar_expect_tx(&full[s], 2 * bytes);
-                    bulk_g2s(dstk, P.kvk + src, bytes, &full[s]);
-                    bulk_g2s(dstk + TILE_BYTES, P.kvv + src, bytes, &full[s]);
+                    bulk_g2s(dstk, (kept ? P.sink.k : P.kvk) + src, bytes, &full[s]);
+                    bulk_g2s(dstk + TILE_BYTES, (kept ? P.sink.v : P.kvv) + src, bytes, &full[s]);
                 }
                 g += pc.n;
             }
@@ -244,7 +248,7 @@ k_flash_decode(const Params P) {
         int cnt = 0;
         for (int g = g0; g < g1;) {
             const Piece pc = locate(g, g1, cum, P.n_seq, P.Hkv);
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
                                           P.n_slots, P.status);
             const int item = pc.i * P.Hkv + pc.kvh;
 
@@ -302,9 +306,9 @@ k_flash_decode(const Params P) {
                 for (int e = 0; e < 2; ++e) {
                     const int r = min((nt * 8 + 2 * t4 + e) / P.G, P.rows - 1);
                     lim[nt][e] = sr.p0 + r;                                       // bruce.cu:2056
-                    low[nt][e] = P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;      // bruce.cu:3688
+                    low[nt][e] = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;      // bruce.cu:3688
                 }
-            const int full_lo = P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;      // window start of the last row
+            const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;      // window start of the last row
 
             float m[NT][2], l[NT][2], O[NBLK][2][NT][4];
 #pragma unroll
@@ -319,7 +323,7 @@ k_flash_decode(const Params P) {
                         for (int c = 0; c < 4; ++c) O[b][u][nt][c] = 0.f;
             }
 
-            const int tile0 = sr.lo / TILE + pc.tl;
+            const KeyTiles<VAR, TILE> kt(sr.lo, P.sink);
             for (int t = 0; t < pc.n; ++t, ++cnt) {
                 const int s = cnt % STAGES, use = cnt / STAGES;
                 if (!*(volatile int*)&s_abort) {
@@ -330,7 +334,7 @@ k_flash_decode(const Params P) {
                 }
                 const uint8_t* Kt = stages + (size_t)s * 2 * TILE_BYTES;
                 const uint8_t* Vt = Kt + TILE_BYTES;
-                const int t0 = (tile0 + t) * TILE;
+                const int t0 = kt.at(pc.tl + t) * TILE;
                 if (AP && sr.p0 >= t0 && sr.p0 < t0 + TILE) {
                     // the tile of the call's own row: warp 0 writes the K record, warp 1 the V record
                     if (warp < 2) {
@@ -364,7 +368,7 @@ k_flash_decode(const Params P) {
                     named_bar_sync(1, NW * 32);
                 }
                 // tiles every row sees completely take the mask-free path (bruce.cu:2927-2928)
-                const bool masked = !(t0 >= full_lo && t0 + TILE - 1 <= sr.p0);
+                const bool masked = !(tile_in_window<VAR, TILE>(t0, full_lo, P.sink) && t0 + TILE - 1 <= sr.p0);
 
                 // ---------------- S^T = K Q^T : 16 keys x (8*NT) pairs --------------------------------
                 float sv[NT][4];
@@ -427,8 +431,8 @@ k_flash_decode(const Params P) {
                         float v0 = sv[nt][e] * P.scale_log2, v1 = sv[nt][2 + e] * P.scale_log2;
                         if (masked) {
                             const int key0 = t0 + kl0, key1 = t0 + kl1;
-                            if (key0 > lim[nt][e] || key0 < low[nt][e]) v0 = NEG_BIG;
-                            if (key1 > lim[nt][e] || key1 < low[nt][e]) v1 = NEG_BIG;
+                            if (key0 > lim[nt][e] || below_window<VAR>(key0, low[nt][e], P.sink)) v0 = NEG_BIG;
+                            if (key1 > lim[nt][e] || below_window<VAR>(key1, low[nt][e], P.sink)) v1 = NEG_BIG;
                         }
                         float mx = fmaxf(v0, v1);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
@@ -488,10 +492,10 @@ k_flash_decode(const Params P) {
                         if (masked) {
                             // keys outside [lo, hi) were never written for this sequence: their bytes
                             // are arbitrary, so their V scale is forced to zero (their P is zero too)
-                            const bool okA = t0 + klA >= sr.lo && t0 + klA < sr.hi;
-                            const bool okB = t0 + klB >= sr.lo && t0 + klB < sr.hi;
-                            const bool okC = t0 + klC >= sr.lo && t0 + klC < sr.hi;
-                            const bool okD = t0 + klD >= sr.lo && t0 + klD < sr.hi;
+                            const bool okA = !below_window<VAR>(t0 + klA, sr.lo, P.sink) && t0 + klA < sr.hi;
+                            const bool okB = !below_window<VAR>(t0 + klB, sr.lo, P.sink) && t0 + klB < sr.hi;
+                            const bool okC = !below_window<VAR>(t0 + klC, sr.lo, P.sink) && t0 + klC < sr.hi;
+                            const bool okD = !below_window<VAR>(t0 + klD, sr.lo, P.sink) && t0 + klD < sr.hi;
 #pragma unroll
                             for (int j = 0; j < NBLK / 2; ++j) {
                                 if (!okA) wa[j] = 0u;

@@ -76,7 +76,30 @@ struct Params {
     // griddepcontrol.wait, i.e. while the append of the chunk's own rows is still running; Q, the tiles holding the
     // chunk's rows and every write come after it (same contract as fd::Params::early)
     int early = 0;
+    // The variants (template parameter VAR) find their sequence on the device, so that idle ones can be skipped:
+    // kslot / act as in the decode calls, or null (slot base pointers, always active)
+    const int* kslot = nullptr;
+    const int* act = nullptr;
+    int n_slots = 1;
+    SinkView sink;               // VAR_SINK
+    // VAR_TRACK: the softmax statistics of every (row, head) in log2 units, with the denominator summed in fp32 from the
+    // unrounded weights (the weights that are accumulated divide by it; the output divides by the sum of the rounded ones).
+    // One split: lse [row][head] = m + log2(l).  Several: stats [split][row][head] = (m, l), joined by the merge.
+    float2* stats = nullptr;
+    float* lse = nullptr;
 };
+// the partition (or table row) of a variant's sequence; -1: idle or bad, nothing to do
+template <int VAR>
+__device__ __forceinline__ int chunk_slot(const Params& P, bool report) {
+    if (VAR == VAR_PLAIN) return P.slot;
+    if (P.act && P.act[0] == 0) return -1;
+    const int s = P.kslot ? P.kslot[0] : P.slot;
+    if (P.kslot && (s < 0 || s >= P.n_slots)) {
+        if (report) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
+        return -1;
+    }
+    return s;
+}
 
 template <int HD, int BN>
 struct Cfg {
@@ -244,7 +267,7 @@ template <int N> __device__ __forceinline__ void regs_grow() { asm volatile("set
 template <int N> __device__ __forceinline__ void regs_shrink() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-template <int HD, int BN>
+template <int HD, int BN, int VAR = VAR_PLAIN>
 __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
     using C = Cfg<HD, BN>;
     constexpr int NBLK = C::NBLK, REC = C::REC;
@@ -273,16 +296,18 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         return;
     }
+    const int kv_slot = chunk_slot<VAR>(P, tid == 0);
+    if (VAR != VAR_PLAIN && kv_slot < 0) return;
     const int rbase = mt * MR;
     const int rows_eff = min(MR, P.rows - rbase);
     const int p_first = p0 + rbase, p_last = p_first + rows_eff - 1;
-    const int lo_cta = P.is_swa ? max(0, p_first + 1 - P.W) : 0;       // bruce.cu:2801
+    const int lo_cta = VAR == VAR_SINK || P.is_swa ? max(0, p_first + 1 - P.W) : 0;       // bruce.cu:2801
     const int hi_cta = p_last + 1;
-    const int full_lo = P.is_swa ? max(0, p_last + 1 - P.W) : 0;
-    const int tile_lo = lo_cta / BN;
-    const int n_all = (hi_cta + BN - 1) / BN - tile_lo;                // key tiles of this M tile
+    const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, p_last + 1 - P.W) : 0;
+    const KeyTiles<VAR, BN> kt(lo_cta, P.sink);
+    const int n_all = kt.count(hi_cta);                                // key tiles of this M tile
     const int per_split = (n_all + P.nsplit - 1) / P.nsplit;
-    const int tile_first = tile_lo + (int)blockIdx.z * per_split;      // this CTA's share
+    const int u_first = (int)blockIdx.z * per_split;                   // this CTA's share: tiles kt.at(u_first + j)
     const int n_tiles = max(0, min(per_split, n_all - (int)blockIdx.z * per_split));
     if (n_tiles == 0) {
         // more splits than key tiles (shallow context): an empty record, so the merge ignores this share
@@ -291,6 +316,8 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
             float* rec = P.recs + ((((size_t)blockIdx.z * P.rows) + rbase + tid / G) * P.Hq + kvh * G + tid % G) * (size_t)(HD + 2);
             for (int i = 0; i < HD; ++i) rec[i] = 0.f;
             rec[HD] = NEG_BIG; rec[HD + 1] = 0.f;
+            if (VAR == VAR_TRACK)
+                P.stats[((size_t)blockIdx.z * P.rows + rbase + tid / G) * P.Hq + kvh * G + tid % G] = make_float2(NEG_BIG, 0.f);
         }
         return;
     }
@@ -391,7 +418,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         }
     };
 
-    const size_t hb = (size_t)kvh * P.pstride * (size_t)REC;
+    const size_t hb = ((size_t)(VAR == VAR_PLAIN ? 0 : kv_slot) * P.Hkv + kvh) * P.pstride * (size_t)REC;
 
     if (warp >= (NSOFT + 2 * NDEQ) / 32) regs_shrink<REGS_CTL>();          // the whole last warpgroup
     if (warp == (NSOFT + 2 * NDEQ) / 32) {
@@ -453,18 +480,21 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
             for (int j = 0; j < n_tiles; ++j) {
                 const int b = j % C::RAW_STAGES;
                 // early streaming stops at the first tile that holds a row of this chunk
-                if (!waited && (tile_first + j + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
+                const int tile = kt.at(u_first + j);
+                if (!waited && (tile + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
                 if (j >= C::RAW_STAGES) wait(B_RAW_FREE0 + b, (j / C::RAW_STAGES - 1) & 1);   // both dequant groups left it
-                const int sp = ((tile_first + j) * BN) & P.ring_mask;
-                const int nk = P.pg.table ? BN : min(BN, P.pstride - sp);
+                const int sp = (tile * BN) & P.ring_mask;
+                const bool kept = VAR == VAR_SINK && P.sink.k && tile * BN < P.sink.cap;     // from the sink buffers
+                const int nk = P.pg.table || kept ? BN : min(BN, P.pstride - sp);
                 const uint32_t bytes = (uint32_t)nk * REC;
                 // (a paged look-up here is hidden by the ring: the loader runs RAW_STAGES tiles ahead of the dequant warps)
-                const size_t off = P.pg.table ? kv_rec_index(P.pg, P.slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
+                const size_t off = P.pg.table ? kv_rec_index(P.pg, kv_slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
+                                 : kept ? (((size_t)kv_slot * P.Hkv + kvh) * P.sink.cap + tile * BN) * (size_t)REC
                                               : hb + (size_t)sp * REC;
                 uint8_t* dst = RAW + b * 2 * C::RAW_BYTES;
                 mbar_expect_tx(&bars[B_RAW_FULL0 + b], 2 * bytes);
-                bulk_g2s(dst, P.kvk + off, bytes, &bars[B_RAW_FULL0 + b]);
-                bulk_g2s(dst + C::RAW_BYTES, P.kvv + off, bytes, &bars[B_RAW_FULL0 + b]);
+                bulk_g2s(dst, (kept ? P.sink.k : P.kvk) + off, bytes, &bars[B_RAW_FULL0 + b]);
+                bulk_g2s(dst + C::RAW_BYTES, (kept ? P.sink.v : P.kvv) + off, bytes, &bars[B_RAW_FULL0 + b]);
             }
         }
     } else if (warp > (NSOFT + 2 * NDEQ) / 32 + 2) {
@@ -483,7 +513,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
 
         for (int j = 0; j < n_tiles; ++j) {
             const int b = j % C::RAW_STAGES;
-            const int t0 = (tile_first + j) * BN;
+            const int t0 = kt.at(u_first + j) * BN;
             const uint8_t* Vraw = RAW + b * 2 * C::RAW_BYTES + C::RAW_BYTES;
             wait(B_RAW_FULL0 + b, (j / C::RAW_STAGES) & 1);
             // the P.V MMA that last read this V buffer (tile j - KV_BUFS) must be complete
@@ -494,7 +524,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                 // so their scale is forced to zero (their P is zero as well)
                 bool kok[8];
 #pragma unroll
-                for (int jj = 0; jj < 8; ++jj) kok[jj] = (t0 + vkey[jj] >= lo_cta) && (t0 + vkey[jj] < hi_cta);
+                for (int jj = 0; jj < 8; ++jj) kok[jj] = !below_window<VAR>(t0 + vkey[jj], lo_cta, P.sink) && (t0 + vkey[jj] < hi_cta);
                 uint32_t sp[4];
 #pragma unroll 1
                 for (int it = 0; it < UPT; ++it) {
@@ -584,18 +614,19 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         const int r = m / G, h = m - r * G;
         const bool row_ok = r < rows_eff;
         const int prow = p_first + r;
-        const int row_lo = P.is_swa ? max(0, prow + 1 - P.W) : 0;     // bruce.cu:3014
+        const int row_lo = VAR == VAR_SINK || P.is_swa ? max(0, prow + 1 - P.W) : 0;     // bruce.cu:3014
         const float c2 = P.scale_log2;
         const float thr = RESCALE_THRESHOLD / c2;              // threshold in raw-score units
         float m_ref = NEG_BIG;                                 // reference maximum, raw-score units
+        float l_exact = 0.f;                                   // VAR_TRACK: the same sum, of the unrounded weights
         float l_part = 0.f;                                    // this thread's share of sum(P) when the tensor core cannot keep it
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = (tile_first + j) * BN;
+            const int t0 = kt.at(u_first + j) * BN;
             const uint32_t tS = tmem + lane_base + ((j & 1) ? C::T_S1 : C::T_S0) + half * HC;
             // tiles every row of the CTA sees completely skip the mask code (bruce.cu:2927-2928)
             // (rows past the end of a ragged M tile hold zero queries: whatever they compute is finite and never stored)
-            const bool masked = !(t0 >= full_lo && t0 + BN - 1 <= p_first);
+            const bool masked = !(tile_in_window<VAR, BN>(t0, full_lo, P.sink) && t0 + BN - 1 <= p_first);
             wait(B_S0 + (j & 1), (j >> 1) & 1);
             tc_fence_after();
             // One read of this thread's S columns; they stay in registers for both the maximum and the
@@ -615,7 +646,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
 #pragma unroll 1
                     for (int i = 0; i < 32; ++i) {
                         const int key = t0 + kappa(half * HC + c * 32 + i);
-                        const bool ok = row_ok && key <= prow && key >= row_lo;
+                        const bool ok = row_ok && key <= prow && !below_window<VAR>(key, row_lo, P.sink);
                         bits |= (ok ? 1u : 0u) << i;
                     }
 #pragma unroll
@@ -677,6 +708,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                     }
                     tmem_st_wait();
                 }
+                if (VAR == VAR_TRACK) l_exact *= fast_exp2((m_ref - m_new) * c2);
                 m_ref = m_new;
             }
             // p = 2^(s*c2 - m_ref*c2); a row that has seen no key yet keeps the offset at zero, so its hidden
@@ -693,7 +725,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                 for (int i = 0; i < 32; i += 2) {
                     float e0, e1;
                     ffma2(e0, e1, __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]), c2p, nbp);
-                    const uint32_t ph = pack_h2(fast_exp2(e0), fast_exp2(e1));
+                    e0 = fast_exp2(e0); e1 = fast_exp2(e1);
+                    if (VAR == VAR_TRACK) l_exact += e0 + e1;
+                    const uint32_t ph = pack_h2(e0, e1);
                     if constexpr (!C::L_MMA) {
                         // the denominator sums the fp16-rounded weights the MMA multiplies with V, so that
                         // out = sum(p v) / sum(p) stays a convex combination of the V rows
@@ -721,6 +755,19 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
             xch[half * 128 + m] = l_part;
             named_bar_sync(2 + (warp & 3), 64);
             l = l_part + xch[(half ^ 1) * 128 + m];
+        }
+        if constexpr (VAR == VAR_TRACK) {
+            // the other exchange buffer was last read before the barrier above
+            volatile float* xch = rmax + ((n_tiles & 1) ^ 1) * 256;
+            xch[half * 128 + m] = l_exact;
+            named_bar_sync(2 + (warp & 3), 64);
+            const float le = l_exact + xch[(half ^ 1) * 128 + m];
+            const size_t si = ((size_t)blockIdx.z * P.rows + rbase + r) * P.Hq + kvh * G + h;
+            const bool some = m_ref > 0.5f * NEG_BIG;
+            if (row_ok && half == 0) {
+                if (P.recs) P.stats[si] = make_float2(some ? m_ref * c2 : NEG_BIG, le);
+                else P.lse[si] = m_ref * c2 + log2f(le);
+            }
         }
         const float il = l > 0.f ? 1.f / l : 0.f;
         const size_t oi = (((size_t)(rbase + r)) * P.Hq + kvh * G + h) * HD + half * (HD / 2);

@@ -154,7 +154,7 @@ __device__ __forceinline__ void umma2_commit(uint64_t* bar) {
                  ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-template <bool PAIR>
+template <bool PAIR, int VAR = VAR_PLAIN>
 __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     using L = Lay<PAIR>;
     constexpr int NB = L::NB;
@@ -189,19 +189,21 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         return;
     }
+    const int kv_slot = chunk_slot<VAR>(P, tid == 0);
+    if (VAR != VAR_PLAIN && kv_slot < 0) return;             // both CTAs of a pair alike
     const int rbase = max(mt, 0) * MR;
     const int rows_eff = mt < 0 ? 0 : min(MR, P.rows - rbase);
     const int p_first = p0 + rbase, p_last = p_first + rows_eff - 1;
-    const int full_lo = P.is_swa ? max(0, p_last + 1 - P.W) : 0;
+    const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, p_last + 1 - P.W) : 0;
     // key range of the CTA, or of the pair (both CTAs walk the same tiles)
     const int rbase_lo = PAIR ? max(mt_pair - 1, 0) * MR : rbase;
-    const int lo_cta = P.is_swa ? max(0, p0 + rbase_lo + 1 - P.W) : 0;       // bruce.cu:2801
+    const int lo_cta = VAR == VAR_SINK || P.is_swa ? max(0, p0 + rbase_lo + 1 - P.W) : 0;       // bruce.cu:2801
     const int hi_cta = p0 + min(P.rows, (mt_pair + 1) * MR);
     // key split: gridDim.z CTAs share this (M tile, kv head), each takes a contiguous share of the key tiles
-    const int tile_lo = lo_cta / BN;
-    const int n_all = (hi_cta + BN - 1) / BN - tile_lo;
+    const KeyTiles<VAR, BN> kt(lo_cta, P.sink);
+    const int n_all = kt.count(hi_cta);
     const int per_split = (n_all + P.nsplit - 1) / P.nsplit;
-    const int tile_first = tile_lo + (int)blockIdx.z * per_split;
+    const int u_first = (int)blockIdx.z * per_split;                          // its tiles: kt.at(u_first + j)
     const int n_tiles = max(0, min(per_split, n_all - (int)blockIdx.z * per_split));
     if (n_tiles == 0) {
         // more splits than key tiles (shallow context): an empty record, so the merge ignores this share
@@ -210,6 +212,8 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             float* rec = P.recs + ((((size_t)blockIdx.z * P.rows) + rbase + tid / G) * P.Hq + kvh * G + tid % G) * (size_t)(HD + 2);
             for (int i = 0; i < HD; ++i) rec[i] = 0.f;
             rec[HD] = NEG_BIG; rec[HD + 1] = 0.f;
+            if (VAR == VAR_TRACK)
+                P.stats[((size_t)blockIdx.z * P.rows + rbase + tid / G) * P.Hq + kvh * G + tid % G] = make_float2(NEG_BIG, 0.f);
         }
         return;
     }
@@ -328,7 +332,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     auto slot = [](int j) { return j % NB; };
     auto phase = [](int j) { return (uint32_t)((j / NB) & 1); };
 
-    const size_t hb = (size_t)kvh * P.pstride * (size_t)REC;
+    const size_t hb = ((size_t)(VAR == VAR_PLAIN ? 0 : kv_slot) * P.Hkv + kvh) * P.pstride * (size_t)REC;
 
     if (warp >= W_MMA) {
         regs_shrink<REGS_CTL>();                                   // the whole last warpgroup
@@ -402,16 +406,19 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             bool waited = !early;
             for (int j = 0; j < n_tiles; ++j) {
                 // early streaming stops at the first tile that holds a row of this chunk
-                if (!waited && (tile_first + j + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
+                const int tile = kt.at(u_first + j);
+                if (!waited && (tile + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
                 if (j >= NB) wait(free_ + slot(j), phase(j - NB), 200);         // the dequant group left it (no hurry: the ring is three deep)
-                const int sp = ((tile_first + j) * BN) & P.ring_mask;
-                const int nk = P.pg.table ? BN : min(BN, P.pstride - sp);
+                const int sp = (tile * BN) & P.ring_mask;
+                const bool kept = VAR == VAR_SINK && P.sink.k && tile * BN < P.sink.cap;     // from the sink buffers
+                const int nk = P.pg.table || kept ? BN : min(BN, P.pstride - sp);
                 const uint32_t bytes = (uint32_t)nk * REC;
                 // (a paged look-up here is hidden by the ring: the loader runs three tiles ahead of the dequant warps)
-                const size_t off = P.pg.table ? kv_rec_index(P.pg, P.slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
+                const size_t off = P.pg.table ? kv_rec_index(P.pg, kv_slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
+                                 : kept ? (((size_t)kv_slot * P.Hkv + kvh) * P.sink.cap + tile * BN) * (size_t)REC
                                               : hb + (size_t)sp * REC;
                 mbar_expect_tx(&bars[full + slot(j)], bytes);
-                bulk_g2s(ring + slot(j) * RAW_BYTES, src + off, bytes, &bars[full + slot(j)]);
+                bulk_g2s(ring + slot(j) * RAW_BYTES, (kept ? (isv ? P.sink.v : P.sink.k) : src) + off, bytes, &bars[full + slot(j)]);
             }
         }
     } else if (warp >= W_VDQ) {
@@ -427,7 +434,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         for (int jj = 0; jj < 8; ++jj) vkey[jj] = kappa(8 * cc + jj);
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = (tile_first + j) * BN;
+            const int t0 = kt.at(u_first + j) * BN;
             const uint8_t* Vraw = smem + OFF_RAWV + slot(j) * RAW_BYTES;
             wait(B_VRAW_FULL + slot(j), phase(j), 50);
             // the P.V MMA that last read this V buffer (tile j - NB) must be complete
@@ -437,7 +444,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             // so their scale is forced to zero (their P is zero as well)
             bool kok[8];
 #pragma unroll
-            for (int jj = 0; jj < 8; ++jj) kok[jj] = (t0 + vkey[jj] >= lo_cta) && (t0 + vkey[jj] < hi_cta);
+            for (int jj = 0; jj < 8; ++jj) kok[jj] = !below_window<VAR>(t0 + vkey[jj], lo_cta, P.sink) && (t0 + vkey[jj] < hi_cta);
             uint32_t sp[4];
 #pragma unroll
             for (int it = 0; it < UPT; ++it) {
@@ -532,21 +539,22 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         const int r = m / G, h = m - r * G;
         const bool row_ok = r < rows_eff;
         const int prow = p_first + r;
-        const int row_lo = P.is_swa ? max(0, prow + 1 - P.W) : 0;     // bruce.cu:3014
+        const int row_lo = VAR == VAR_SINK || P.is_swa ? max(0, prow + 1 - P.W) : 0;     // bruce.cu:3014
         const float c2 = P.scale_log2;
         const float thr = RESCALE_THRESHOLD / c2;              // threshold in raw-score units
         const uint64_t c2p = pack_f2(c2, c2);
         // the two threads of a row keep the row reference in a register each: they see the same maxima and take
         // the same decisions
         float m_ref = NEG_BIG;
+        float l_exact = 0.f;                                   // VAR_TRACK: this thread's share of the unrounded weights
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = (tile_first + j) * BN;
+            const int t0 = kt.at(u_first + j) * BN;
             const int ch2 = L::schunk((j ^ 1) < n_tiles);          // the tile's second 32 columns (see Lay::scol)
             const uint32_t tS = tmem + lane_base + T_S + L::scol(slot(j));
             // tiles every row of the CTA sees completely skip the mask code (bruce.cu:2927-2928)
             // (rows past the end of a ragged M tile hold zero queries: whatever they compute is finite and never stored)
-            const bool masked = !(t0 >= full_lo && t0 + BN - 1 <= p_first);
+            const bool masked = !(tile_in_window<VAR, BN>(t0, full_lo, P.sink) && t0 + BN - 1 <= p_first);
             wait(B_S + slot(j), phase(j), 50);
             tc_fence_after();
             uint32_t v[32];
@@ -560,7 +568,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
 #pragma unroll 1
                 for (int i = 0; i < 32; ++i) {
                     const int key = t0 + kappa(grp * 32 + i);
-                    const bool ok = row_ok && key <= prow && key >= row_lo;
+                    const bool ok = row_ok && key <= prow && !below_window<VAR>(key, row_lo, P.sink);
                     bits |= (ok ? 1u : 0u) << i;
                 }
 #pragma unroll
@@ -613,6 +621,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
                     tmem_st_wait();
                     tc_fence_before();
                 }
+                if (VAR == VAR_TRACK && need) l_exact *= fast_exp2((m_ref - m_new) * c2);
                 if (need) m_ref = m_new;
             }
             // p = 2^(s*c2 - m_ref*c2); a row that has seen no key yet keeps the offset at zero, so its hidden
@@ -627,7 +636,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             for (int i = 0; i < 32; i += 2) {
                 float e0, e1;
                 ffma2(e0, e1, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), c2p, nbp);
-                pk[i >> 1] = pack_h2(fast_exp2(e0), fast_exp2(e1));
+                e0 = fast_exp2(e0); e1 = fast_exp2(e1);
+                if (VAR == VAR_TRACK) l_exact += e0 + e1;
+                pk[i >> 1] = pack_h2(e0, e1);
             }
             tmem_st16(tS + 16 * grp, pk);
             tmem_st_wait();
@@ -641,6 +652,19 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         wait(B_PV + slot(n_tiles - 1), phase(n_tiles - 1), 50);
         tc_fence_after();
         const float l = __uint_as_float(tmem_ld1(tmem + lane_base + T_L));
+        if constexpr (VAR == VAR_TRACK) {
+            // the two threads of a row add their shares; the exchange buffer of the opposite tile parity is idle
+            volatile float* x = mref + (n_tiles & 1) * 256;
+            x[grp * 128 + m] = l_exact;
+            named_bar_sync(4 + qtr, 64);
+            const float le = l_exact + x[(grp ^ 1) * 128 + m];
+            const size_t si = ((size_t)blockIdx.z * P.rows + rbase + r) * P.Hq + kvh * G + h;
+            const bool some = m_ref > 0.5f * NEG_BIG;
+            if (row_ok && grp == 0) {
+                if (P.recs) P.stats[si] = make_float2(some ? m_ref * c2 : NEG_BIG, le);
+                else P.lse[si] = m_ref * c2 + log2f(le);
+            }
+        }
         const float il = l > 0.f ? 1.f / l : 0.f;
         const size_t oi = (((size_t)(rbase + r)) * P.Hq + kvh * G + h) * HD + grp * (HD / 2);
         // with key splits: a split record (unnormalised o, m in log2 units, l) instead of the output row

@@ -49,7 +49,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* 
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
 }
 
-template <int HD>
+template <int HD, int VAR = VAR_PLAIN>
 __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(const fd::Params P) {
     using C = Cfg<HD>;
     constexpr int NBLK = C::NBLK, REC = C::REC, TILE_BYTES = C::TILE_BYTES, HSTR = C::HSTR;
@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
     if (P.epoch_ptr && blockIdx.x == 0 && tid == 0) *P.epoch_ptr += P.epoch_advance;
     // ---- the flash-decode work cut: every CTA derives the same tile shares from the positions -------
     for (int i = tid; i < P.n_seq; i += NTHREADS) {
-        const SeqRange sr = seq_range(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
-        cum[i + 1] = sr.active ? ((sr.hi + TILE - 1) / TILE - sr.lo / TILE) : 0;
+        const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+        cum[i + 1] = sr.active ? KeyTiles<VAR, TILE>(sr.lo, P.sink).count(sr.hi) : 0;
     }
     if (tid == 0) cum[0] = 0;
     __syncthreads();
@@ -113,17 +113,17 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
             int cnt = 0;
             for (int g = g0; g < g1;) {
                 const fd::Piece pc = fd::locate(g, g1, cum, P.n_seq, P.Hkv);
-                const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
+                const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
                                               P.n_slots, P.status);
                 const size_t hb = ((size_t)sr.slot * P.Hkv + pc.kvh) * P.pstride * (size_t)REC;
-                const int tile0 = sr.lo / TILE + pc.tl;
+                const KeyTiles<VAR, TILE> kt(sr.lo, P.sink);
                 // paged cache: the table entry of the next tile is fetched one tile ahead of its use
                 const int* trow = P.pg.table ? P.pg.table + (size_t)sr.slot * P.pg.max_pages : nullptr;
-                int page_nx = trow ? trow[(tile0 * TILE) >> P.pg.shift] : 0;
+                int page_nx = trow ? trow[(kt.at(pc.tl) * TILE) >> P.pg.shift] : 0;
                 for (int t = 0; t < pc.n; ++t, ++cnt) {
                     const int s = cnt % STAGES, use = cnt / STAGES;
-                    const int page = page_nx;
-                    if (trow && t + 1 < pc.n) page_nx = trow[((tile0 + t + 1) * TILE) >> P.pg.shift];
+                    const int page = page_nx, tile = kt.at(pc.tl + t);
+                    if (trow && t + 1 < pc.n) page_nx = trow[(kt.at(pc.tl + t + 1) * TILE) >> P.pg.shift];
                     if (use > 0 && !*(volatile int*)&s_abort) {
                         if (!mbar_wait_bounded(&empty[s], (use - 1) & 1)) {
                             atomicOr(P.status, BATTN_DEV_WAIT_TIMEOUT);
@@ -131,15 +131,17 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
                         }
                     }
                     if (*(volatile int*)&s_abort) continue;
-                    const int sp = ((tile0 + t) * TILE) & P.ring_mask;
-                    const int nk = trow ? TILE : min(TILE, P.pstride - sp);
+                    const int sp = (tile * TILE) & P.ring_mask;
+                    const bool kept = VAR == VAR_SINK && P.sink.k && tile * TILE < P.sink.cap;   // from the sink buffers
+                    const int nk = trow || kept ? TILE : min(TILE, P.pstride - sp);
                     const uint32_t bytes = (uint32_t)nk * REC;
                     const size_t src = trow ? kv_rec_index_page(P.pg, page, pc.kvh, P.Hkv, sp, P.status) * (size_t)REC
+                                     : kept ? (((size_t)sr.slot * P.Hkv + pc.kvh) * P.sink.cap + tile * TILE) * (size_t)REC
                                             : hb + (size_t)sp * REC;
                     uint8_t* dstk = stages + (size_t)s * 2 * TILE_BYTES;
                     mbar_expect_tx(&full[s], 2 * bytes);
-                    bulk_g2s(dstk, P.kvk + src, bytes, &full[s]);
-                    bulk_g2s(dstk + TILE_BYTES, P.kvv + src, bytes, &full[s]);
+                    bulk_g2s(dstk, (kept ? P.sink.k : P.kvk) + src, bytes, &full[s]);
+                    bulk_g2s(dstk + TILE_BYTES, (kept ? P.sink.v : P.kvv) + src, bytes, &full[s]);
                 }
                 g += pc.n;
             }
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
         int cnt = 0;
         for (int g = g0; g < g1;) {
             const fd::Piece pc = fd::locate(g, g1, cum, P.n_seq, P.Hkv);
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx,
                                           P.n_slots, P.status);
             const int item = pc.i * P.Hkv + pc.kvh;
 
@@ -189,16 +191,16 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
             for (int e = 0; e < 2; ++e) {
                 const int r = min((pair0 + 2 * t4 + e) / P.G, P.rows - 1);
                 lim[e] = sr.p0 + r;                                            // bruce.cu:2056
-                low[e] = P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;           // bruce.cu:3688
+                low[e] = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;           // bruce.cu:3688
             }
-            const int full_lo = P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;
+            const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;
 
             float m[2] = {NEG_BIG, NEG_BIG}, l[2] = {0.f, 0.f};
             float O[HD / 16][4];                                               // O^T: 16-dim tiles x (2 dims x 2 pairs)
 #pragma unroll
             for (int dt = 0; dt < HD / 16; ++dt) O[dt][0] = O[dt][1] = O[dt][2] = O[dt][3] = 0.f;
 
-            const int tile0 = sr.lo / TILE + pc.tl;
+            const KeyTiles<VAR, TILE> kt(sr.lo, P.sink);
             for (int t = 0; t < pc.n; ++t, ++cnt) {
                 const int s = cnt % STAGES, use = cnt / STAGES;
                 if (!*(volatile int*)&s_abort) {
@@ -209,8 +211,8 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
                 }
                 const uint8_t* Kt = stages + (size_t)s * 2 * TILE_BYTES;
                 const uint8_t* Vt = Kt + TILE_BYTES;
-                const int t0 = (tile0 + t) * TILE;
-                const bool masked = !(t0 >= full_lo && t0 + TILE - 1 <= sr.p0);
+                const int t0 = kt.at(pc.tl + t) * TILE;
+                const bool masked = !(tile_in_window<VAR, TILE>(t0, full_lo, P.sink) && t0 + TILE - 1 <= sr.p0);
 
                 named_bar_sync(1, NW * 32);          // every warp is done with the previous fp16 tile
                 // ---------------- convert this warp's 16 keys: 8-byte chunks, 16 per key -----------------
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
                     const uint2 kw = *reinterpret_cast<const uint2*>(kr + 2 * NBLK + ch * 8);
                     const uint2 vw = *reinterpret_cast<const uint2*>(vr + 2 * NBLK + ch * 8);
                     __half dv = reinterpret_cast<const __half*>(vr)[ch >> 2];
-                    if (masked && (t0 + key < sr.lo || t0 + key >= sr.hi)) dv = __float2half_rn(0.f);   // never-written slot
+                    if (masked && (below_window<VAR>(t0 + key, sr.lo, P.sink) || t0 + key >= sr.hi)) dv = __float2half_rn(0.f);   // never-written slot
                     const __half2 d2 = __half2half2(dv);
                     const uint32_t du = *reinterpret_cast<const uint32_t*>(&d2);
                     const uint32_t kx = kw.x ^ 0x80808080u, ky = kw.y ^ 0x80808080u;
@@ -273,8 +275,8 @@ __global__ void __launch_bounds__(NTHREADS, HD == 128 ? 3 : 1) k_verify_wide(con
                         float v0 = sv[mt][e] * P.scale_log2, v1 = sv[mt][2 + e] * P.scale_log2;
                         if (masked) {
                             const int key0 = t0 + mt * 16 + gid, key1 = key0 + 8;
-                            if (key0 > lim[e] || key0 < low[e]) v0 = NEG_BIG;
-                            if (key1 > lim[e] || key1 < low[e]) v1 = NEG_BIG;
+                            if (key0 > lim[e] || below_window<VAR>(key0, low[e], P.sink)) v0 = NEG_BIG;
+                            if (key1 > lim[e] || below_window<VAR>(key1, low[e], P.sink)) v1 = NEG_BIG;
                         }
                         sv[mt][e] = v0; sv[mt][2 + e] = v1;
                         mx[e] = fmaxf(mx[e], fmaxf(v0, v1));

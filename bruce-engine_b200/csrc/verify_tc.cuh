@@ -149,6 +149,7 @@ __device__ __forceinline__ float pick16(const float (&v)[16], int idx) {
     return r;
 }
 
+template <int VAR>
 __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // 1024-byte aligned
@@ -188,8 +189,8 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
     if (P.epoch_ptr && blockIdx.x == 0 && tid == 0) *P.epoch_ptr += P.epoch_advance;
     // ---- the flash-decode work cut in 128-key tiles: every CTA derives the same shares from the positions --------
     for (int i = tid; i < P.n_seq; i += NTHREADS) {
-        const SeqRange sr = seq_range(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
-        cum[i + 1] = sr.active ? ((sr.hi + BK - 1) / BK - sr.lo / BK) : 0;
+        const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+        cum[i + 1] = sr.active ? KeyTiles<VAR, BK>(sr.lo, P.sink).count(sr.hi) : 0;
     }
     if (tid == 0) cum[0] = 0;
     tc_fence_before();
@@ -290,27 +291,29 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
             int cnt = 0;
             for (int g = g0; g < g1;) {
                 const fd::Piece pc = fd::locate(g, g1, cum, P.n_seq, P.Hkv);
-                const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots,
+                const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots,
                                               P.status);
                 const size_t hb = ((size_t)sr.slot * P.Hkv + pc.kvh) * P.pstride * (size_t)REC;
                 const uint8_t* src = isv ? P.kvv : P.kvk;
-                const int tile0 = sr.lo / BK + pc.tl;
+                const KeyTiles<VAR, BK> kt(sr.lo, P.sink);
                 // paged cache: the table entry of the next tile is fetched one tile ahead of its use
                 const int* trow = P.pg.table ? P.pg.table + (size_t)sr.slot * P.pg.max_pages : nullptr;
-                int page_nx = trow ? trow[(tile0 * BK) >> P.pg.shift] : 0;
+                int page_nx = trow ? trow[(kt.at(pc.tl) * BK) >> P.pg.shift] : 0;
                 for (int t = 0; t < pc.n; ++t, ++cnt) {
-                    const int page = page_nx;
-                    if (trow && t + 1 < pc.n) page_nx = trow[((tile0 + t + 1) * BK) >> P.pg.shift];
+                    const int page = page_nx, tile = kt.at(pc.tl + t);
+                    if (trow && t + 1 < pc.n) page_nx = trow[(kt.at(pc.tl + t + 1) * BK) >> P.pg.shift];
                     if (cnt >= NB) wait(free_ + slot(cnt), phase(cnt - NB), 100);
                     if (misc[1]) continue;
                     VT_TRACE(isv ? 3 : 2, cnt, 0);
-                    const int sp = ((tile0 + t) * BK) & P.ring_mask;
-                    const int nk = trow ? BK : min(BK, P.pstride - sp);
+                    const int sp = (tile * BK) & P.ring_mask;
+                    const bool kept = VAR == VAR_SINK && P.sink.k && tile * BK < P.sink.cap;     // from the sink buffers
+                    const int nk = trow || kept ? BK : min(BK, P.pstride - sp);
                     const uint32_t bytes = (uint32_t)nk * REC;
                     const size_t off = trow ? kv_rec_index_page(P.pg, page, pc.kvh, P.Hkv, sp, P.status) * (size_t)REC
+                                     : kept ? (((size_t)sr.slot * P.Hkv + pc.kvh) * P.sink.cap + tile * BK) * (size_t)REC
                                             : hb + (size_t)sp * REC;
                     mbar_expect_tx(&bars[full + slot(cnt)], bytes);
-                    bulk_g2s(ring + slot(cnt) * RAW_BYTES, src + off, bytes, &bars[full + slot(cnt)]);
+                    bulk_g2s(ring + slot(cnt) * RAW_BYTES, (kept ? (isv ? P.sink.v : P.sink.k) : src) + off, bytes, &bars[full + slot(cnt)]);
                 }
                 g += pc.n;
             }
@@ -329,10 +332,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
         int cnt = 0;
         for (int g = g0; g < g1;) {
             const fd::Piece pc = fd::locate(g, g1, cum, P.n_seq, P.Hkv);
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
-            const int tile0 = sr.lo / BK + pc.tl;
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+            const KeyTiles<VAR, BK> kt(sr.lo, P.sink);
             for (int tt = 0; tt < pc.n; ++tt, ++cnt) {
-                const int t0 = (tile0 + tt) * BK;
+                const int t0 = kt.at(pc.tl + tt) * BK;
                 const uint8_t* Vraw = smem + OFF_RAWV + slot(cnt) * RAW_BYTES;
                 wait(B_VRAW_FULL + slot(cnt), phase(cnt), 50);
                 if (t == 0) VT_TRACE(4, cnt, 0);
@@ -343,7 +346,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
                 // their scale is forced to zero (their P is zero as well)
                 bool kok[8];
 #pragma unroll
-                for (int jj = 0; jj < 8; ++jj) kok[jj] = (t0 + vkey[jj] >= sr.lo) && (t0 + vkey[jj] < sr.hi);
+                for (int jj = 0; jj < 8; ++jj) kok[jj] = !below_window<VAR>(t0 + vkey[jj], sr.lo, P.sink) && (t0 + vkey[jj] < sr.hi);
                 uint32_t sp[4];
 #pragma unroll 1
                 for (int it = 0; it < UPT; ++it) {
@@ -449,7 +452,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
         int cnt = 0, piece = 0;
         for (int g = g0; g < g1; ++piece) {
             const fd::Piece pc = fd::locate(g, g1, cum, P.n_seq, P.Hkv);
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+            const SeqRange sr = seq_keys<VAR>(P.pos, P.kslot, P.act, pc.i, P.rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
             const int item = pc.i * P.Hkv + pc.kvh;
             // ---- this item's Q as the B operand [pair][dim]: a thread writes 16 bytes of two pairs ----------------
             // (the previous piece's last S^T product has completed: these threads consumed its result)
@@ -477,7 +480,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars[B_Q]);
             }
-            const int full_lo = P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;      // window start of the last row
+            const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;      // window start of the last row
             // References (log2 units), one per pair, held by EVERY thread of the group.  A reference moves only when
             // some score of a tile exceeds it by more than 2^8 (then to that tile's maximum): weights stay below 2^8,
             // well inside fp16, and on the common tile each thread only checks its own differences.
@@ -494,10 +497,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
                     pcol[r8] = smem_u32(Psm) + (n >> 6) * P_SUB + (pbase >> 3) * 1024 + (((kc ^ r8) & 7) << 4) + kb;
             }
 
-            const int tile0 = sr.lo / BK + pc.tl;
+            const KeyTiles<VAR, BK> kt(sr.lo, P.sink);
             for (int t = 0; t < pc.n; ++t, ++cnt) {
-                const int t0 = (tile0 + t) * BK;
-                const bool masked = !(t0 >= full_lo && t0 + BK - 1 <= sr.p0);
+                const int t0 = kt.at(pc.tl + t) * BK;
+                const bool masked = !(tile_in_window<VAR, BK>(t0, full_lo, P.sink) && t0 + BK - 1 <= sr.p0);
                 wait(B_S + slot(cnt), phase(cnt), 30);
                 tc_fence_after();
                 if (tid == 0) VT_TRACE(6, cnt, 0);
@@ -535,8 +538,8 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_verify_tc(const fd::Params P) {
                     for (int i = 0; i < NPH; ++i) {                    // (i / G folds to a shift per pair for G = 4)
                         const int r = min((pbase + i) / P.G, P.rows - 1);
                         const int lim = sr.p0 + r;                                         // bruce.cu:2056
-                        const int low = P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;        // bruce.cu:3688
-                        if (key > lim || key < low) v[i] = -INFINITY;
+                        const int low = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + r + 1 - P.W) : 0;        // bruce.cu:3688
+                        if (key > lim || below_window<VAR>(key, low, P.sink)) v[i] = -INFINITY;
                     }
                 }
                 // ---- does any score of the tile outgrow its reference?  (own differences, then a vote) --------------

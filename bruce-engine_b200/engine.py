@@ -262,6 +262,69 @@ class AttnEngine:
                                                _ptr(act), _ptr(part), n_seq, rows, nsplit, self._stream())
         self._check("battn_attend_exact_paged", rc)
 
+    # ---- sliding window with sinks ---------------------------------------------------------------------
+    def _dev(self, name: str, t, dtype, n: int = 0):
+        """The pointer of a device tensor the new calls read or write, after the checks a raw pointer cannot have."""
+        if t.dtype is not dtype or not t.is_contiguous() or t.device != self.device or t.numel() < n:
+            raise ValueError(f"{name}: need a contiguous {dtype} tensor of at least {n} elements on {self.device}, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def _seqs(self, pos, sel, act):
+        """Pointers of the per-sequence arrays: positions, partitions (or table rows) and activity."""
+        n = pos.numel()
+        return (self._dev("pos", pos, torch.int32), None if sel is None else self._dev("kslot", sel, torch.int32, n),
+                None if act is None else self._dev("act", act, torch.int32, n), n)
+
+    def _cache_ptrs(self, kvk, kvv, is_swa: bool, layer: bool):
+        """A layer's (or, for the single-sequence form, one slot's) K and V buffers."""
+        g = self.geom
+        n = (g.n_slots if layer else 1) * g.pstride(is_swa) * g.n_kv * g.rec
+        return self._dev("kvk", kvk, torch.uint8, n), self._dev("kvv", kvv, torch.uint8, n)
+
+    def _stream_here(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def alloc_sinks(self, n_sink: int):
+        """Sink buffers of one window layer for all slots; returns (descriptor, k, v): keep the tensors alive with it."""
+        cap, n = max(128, -(-n_sink // 128) * 128), C.c_size_t()
+        self._check("battn_sinks_bytes", self.lib.battn_sinks_bytes(self.h, cap, C.byref(n)))
+        k, v = (torch.zeros(n.value, dtype=torch.uint8, device=self.device) for _ in range(2))
+        return self.sinks(n_sink, k, v), k, v
+
+    def sinks(self, n_sink: int, k=None, v=None):
+        """The descriptor of `n_sink` sinks: over buffers for a ring layer, without for a cache that keeps its first positions."""
+        if (k is None) != (v is None):
+            raise ValueError("sinks: both buffers or neither")
+        if k is None:
+            return capi.CSinks(None, None, n_sink, 0)
+        cap = k.numel() // (self.geom.n_slots * self.geom.n_kv * self.geom.rec)
+        return capi.CSinks(self._dev("k", k, torch.uint8), self._dev("v", v, torch.uint8, k.numel()), n_sink, cap)
+
+    def sinks_store(self, kvk, kvv, sinks, pos, kslot=None, act=None, rows: int = 1):
+        """Behind the append of the same rows: the records of the first positions, ring -> sink buffers."""
+        p, s, a, n = self._seqs(pos, kslot, act)
+        k, v = self._cache_ptrs(kvk, kvv, True, kslot is not None)
+        self._check("battn_sinks_store", self.lib.battn_sinks_store(self.h, k, v, C.byref(sinks), p, s, a, n, rows,
+                                                                    self._stream_here()))
+
+    def attn_sinks(self, out, q, kvk, kvv, sinks, pos, part, rows: int = 1, kslot=None, act=None, is_swa: bool = True):
+        """Sliding-window attention whose rows see the first n_sink positions too: `rows` rows of every sequence (decode,
+        verify) or a prompt chunk of one."""
+        p, s, a, n = self._seqs(pos, kslot, act)
+        k, v = self._cache_ptrs(kvk, kvv, is_swa, kslot is not None)
+        nq = n * rows * self.geom.n_head * self.geom.head_dim
+        self._check("battn_attend_sinks", self.lib.battn_attend_sinks(
+            self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), k, v, C.byref(sinks),
+            p, s, a, part.data_ptr(), rows, n, int(is_swa), self._stream_here()))
+
+    def attn_sinks_paged(self, out, q, pages, sinks, pos, part, rows: int = 1, ktab=None, act=None):
+        p, s, a, n = self._seqs(pos, ktab, act)
+        nq = n * rows * self.geom.n_head * self.geom.head_dim
+        self._check("battn_attend_sinks_paged", self.lib.battn_attend_sinks_paged(
+            self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), C.byref(pages),
+            C.byref(sinks), p, s, a, part.data_ptr(), rows, n, self._stream_here()))
+
     # ---- the step after attention ------------------------------------------------------------------------
     def gate_norm(self, dst, aout, gate, sgate, xq, xd, xsum, rows: int):
         """k_gate_norm_vec4 (bruce.cu:1526): sigmoid gate, L2 norm, q8 activation copy; dst may be None."""

@@ -341,6 +341,43 @@ int battn_attend_exact_paged(battn_handle* h, void* out, const void* q, const ba
                              const int* ktab, const int* act, void* ws, int n_seq, int rows_per_seq, int nsplit,
                              void* stream);
 
+/* ---- Sliding window with sinks -------------------------------------------------------------------------------------
+ * A row at position p sees its window and the first n_sink positions of its sequence:
+ *     key <= p  and  (key > p - window  or  key < n_sink)
+ * (no counterpart in the reference, whose window layers forget their first tokens).  A model that was trained with full
+ * attention keeps its quality over an endless stream when the first few tokens, which draw most of the attention no row
+ * needs elsewhere, stay visible beside the window.  The geometry's window applies.  Three kinds of cache:
+ *   - a ring layer (is_swa = 1): the ring forgets the first positions, so they are kept in sink buffers beside it,
+ *         k, v: [slot][kv head][cap positions][record], battn_sinks_bytes each, cap a multiple of 128, >= n_sink
+ *     which hold the first `cap` positions of every sequence.  battn_sinks_store copies them from the ring; call it after
+ *     every append until the sequence is longer than cap (later calls do nothing, so it may stay in a captured step).
+ *     EVERY key below cap is read from the sink buffers, those of a sequence that still fits the ring too.
+ *   - a full layer (is_swa = 0) and a paged cache: the first positions are where they always were; k = v = NULL.  Page
+ *     table entries of pages that lie wholly between the sinks and the window are never read and may be -1.
+ * n_sink is 0 .. window. */
+typedef struct battn_sinks {
+    uint8_t* k;
+    uint8_t* v;
+    int n_sink, cap;
+} battn_sinks;
+int battn_sinks_bytes(const battn_handle* h, int cap, size_t* out_bytes);
+/* The records of positions pos[i] .. pos[i]+rows_per_seq-1 that lie below cap, ring -> sink buffers.  The rows must still
+ * be in the ring: call it behind the append of exactly these rows.  pos, kslot, act as battn_kv_append; kslot == NULL:
+ * kvk, kvv and the sink buffers are the slot's bases. */
+int battn_sinks_store(battn_handle* h, const uint8_t* kvk, const uint8_t* kvv, const battn_sinks* sinks, const int* pos,
+                      const int* kslot, const int* act, int n_seq, int rows_per_seq, void* stream);
+/* Attention of `rows` rows per sequence at pos[i] .. pos[i]+rows-1, whose records are in the cache:
+ *   rows * (n_head / n_kv) <= 32 and rows <= 8: n_seq sequences, as battn_decode (1 row) and battn_verify
+ *   more rows, up to 512: a prompt chunk of one sequence (n_seq = 1), as battn_prefill
+ *   q, out [n_seq][rows][n_head][head_dim]; ws: battn_workspace_bytes(n_seq, rows).
+ *   kslot / act (ktab) as in those calls; a prompt chunk may name its partition by kslot too.  Sequences with
+ *   act[i] == 0 or a bad position produce no output. */
+int battn_attend_sinks(battn_handle* h, void* out, const void* q, const uint8_t* kvk, const uint8_t* kvv,
+                       const battn_sinks* sinks, const int* pos, const int* kslot, const int* act, void* ws, int rows,
+                       int n_seq, int is_swa, void* stream);
+int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const battn_pages* pages, const battn_sinks* sinks,
+                             const int* pos, const int* ktab, const int* act, void* ws, int rows, int n_seq, void* stream);
+
 /* ---- One sequence split by position range across several devices (no counterpart in the reference, which is
  * single-GPU; built on its split record and merge, bruce.cu:781-783, 992-1007) ------------------------------------
  * Device r of `world` holds positions [r*N/world, (r+1)*N/world) of the sequence in its own cache, with LOCAL
