@@ -81,6 +81,9 @@ SIGNATURES = {
     "battn_sinks_store": (_I, [_P, _P, _P, _SK] + [_P] * 3 + [_I, _I, _P]),
     "battn_attend_sinks": (_I, [_P] * 5 + [_SK] + [_P] * 4 + [_I, _I, _I, _P]),
     "battn_attend_sinks_paged": (_I, [_P] * 3 + [_PG, _SK] + [_P] * 4 + [_I, _I, _P]),
+    "battn_evict_workspace_bytes": (_I, [_P, _I, _SZP]),
+    "battn_evict": (_I, [_P] * 11 + [_I] * 4 + [_P]),
+    "battn_evict_paged": (_I, [_P, _PG] + [_P] * 8 + [_I] * 4 + [_P]),
     "battn_xchg_create": (_I, [_P, _I, _I, _I, C.POINTER(_P), _P]),
     "battn_xchg_connect": (_I, [_P, _P]),
     "battn_xchg_area": (_I, [_P, C.POINTER(_P), _SZP]),

@@ -7,6 +7,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "evict.cuh"
 #include "exact.cuh"
 #include "flash_decode.cuh"
 #include "gate_norm.cuh"
@@ -97,6 +98,8 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     } else {
         if ((e = allow_smem(pf::k_prefill<256, 64, VAR_SINK>, pf::Cfg<256, 64>::TOTAL)) != cudaSuccess) return e;
     }
+    if ((e = allow_smem(ev::k_evict_select, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
+    if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::SMEM)) != cudaSuccess) return e;
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 2, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
@@ -988,6 +991,78 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
     const int rc = paged_view(pages, pv);
     if (rc) return rc;
     return attend_sinks_impl(h, out, q, pages->pool_k, pages->pool_v, sinks, pos, ktab, act, ws, rows, n_seq, 0, stream, &pv);
+}
+
+// ---- eviction by accumulated attention weight ------------------------------------------------------------------
+int battn_evict_workspace_bytes(const battn_handle* h, int n_seq, size_t* out_bytes) {
+    if (!h || !out_bytes || n_seq < 1) return BATTN_ERR_ARG;
+    if (n_seq > MAX_SEQ) return BATTN_ERR_CAPACITY;
+    *out_bytes = align_up((size_t)n_seq * sizeof(int), 256);
+    return BATTN_OK;
+}
+
+// CTAs per cluster for `items` clusters: as many as the SMs have room for, a power of two up to the portable limit
+static int evict_cluster(const battn_handle* h, int items) {
+    int c = 1;
+    while (c < ev::MAX_CLUSTER && items * c * 2 <= h->num_sms) c *= 2;
+    return c;
+}
+
+static int evict_impl(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score, int* kept, int* pos_out, const int* pos,
+                      const int* kslot, const int* kslot_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
+                      int n_seq, void* stream, const PagedView* pv) {
+    const int rc = check_seq_args(h, kvk, kvv, score, kept, pos, kslot, n_seq, 1, 1);
+    if (rc) return rc;
+    if (!pos_out || !ws || ((uintptr_t)ws & 15) || (!kslot && kslot_dst)) return BATTN_ERR_ARG;
+    const Geom& g = h->g;
+    if (budget < 1 || n_sink < 0 || n_recent < 0 || n_sink > budget || n_recent > budget - n_sink) return BATTN_ERR_ARG;
+    ev::Params P;
+    P.kvk = kvk; P.kvv = kvv; P.score = score; P.kept = kept; P.pos_out = pos_out; P.plan = reinterpret_cast<int*>(ws);
+    P.pos = pos; P.kslot = kslot; P.kslot_dst = kslot_dst; P.act = act;
+    P.n_seq = n_seq; P.budget = budget; P.n_sink = n_sink; P.n_recent = n_recent;
+    P.Hkv = g.Hkv; P.pstride = g.slot_ctx; P.n_slots = g.n_slots; P.status = h->d_status;
+    if (pv) { P.pg = pv->pg; P.pstride = pv->capacity; P.n_slots = pv->n_tables; }
+    if (budget > P.pstride) return BATTN_ERR_CAPACITY;
+    const DeviceScope dev(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    h->kvw_kind = 2;                     // the records of every position may have moved
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2; cfg.stream = st;
+    int c = evict_cluster(h, n_seq * g.Hkv);
+    attr[0].val.clusterDim.x = c;
+    cfg.gridDim = dim3(n_seq * c, g.Hkv); cfg.blockDim = dim3(ev::SEL_THREADS); cfg.dynamicSmemBytes = ev::KEYS_SMEM * 4;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, ev::k_evict_select, P);
+    if (e != cudaSuccess) return cuda_fail(h, e);
+    c = evict_cluster(h, n_seq * g.Hkv * 2);
+    attr[0].val.clusterDim.x = c;
+    cfg.gridDim = dim3(n_seq * c, g.Hkv, 2); cfg.blockDim = dim3(ev::MOVE_THREADS);
+    cfg.dynamicSmemBytes = g.HD == 128 ? ev::MoveCfg<128>::SMEM : ev::MoveCfg<256>::SMEM;
+    e = g.HD == 128 ? cudaLaunchKernelEx(&cfg, ev::k_evict_move<128>, P) : cudaLaunchKernelEx(&cfg, ev::k_evict_move<256>, P);
+    h->launches += 2;
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? BATTN_OK : cuda_fail(h, e);
+}
+
+int battn_evict(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score, int* kept, int* pos_out, const int* pos,
+                const int* kslot, const int* kslot_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
+                int n_seq, void* stream) {
+    return evict_impl(h, kvk, kvv, score, kept, pos_out, pos, kslot, kslot_dst, act, ws, budget, n_sink, n_recent, n_seq, stream,
+                      nullptr);
+}
+
+int battn_evict_paged(battn_handle* h, const battn_pages* pages, float* score, int* kept, int* pos_out, const int* pos,
+                      const int* ktab, const int* ktab_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
+                      int n_seq, void* stream) {
+    PagedView pv;
+    const int rc = paged_view(pages, pv);
+    if (rc) return rc;
+    return evict_impl(h, pages->pool_k, pages->pool_v, score, kept, pos_out, pos, ktab, ktab_dst, act, ws, budget, n_sink,
+                      n_recent, n_seq, stream, &pv);
 }
 
 int battn_xchg_create(battn_handle* h, int rank, int world, int max_rows, battn_xchg** out_x, void* ipc_handle_out) {

@@ -325,6 +325,36 @@ class AttnEngine:
             self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), C.byref(pages),
             C.byref(sinks), p, s, a, part.data_ptr(), rows, n, self._stream_here()))
 
+    # ---- eviction by accumulated attention weight --------------------------------------------------------
+    def alloc_evict_part(self, n_seq: int) -> torch.Tensor:
+        n = C.c_size_t()
+        self._check("battn_evict_workspace_bytes", self.lib.battn_evict_workspace_bytes(self.h, n_seq, C.byref(n)))
+        return torch.empty(n.value, dtype=torch.uint8, device=self.device)
+
+    def _evict_args(self, score, kept, pos_out, pos, part, budget, sel, sel_dst, act, scores: int):
+        p, s, a, n = self._seqs(pos, sel, act)
+        d = None if sel_dst is None else self._dev("kslot_dst", sel_dst, torch.int32, n)
+        return n, (self._dev("score", score, torch.float32, scores),
+                   self._dev("kept", kept, torch.int32, n * self.geom.n_kv * max(budget, 1)),
+                   self._dev("pos_out", pos_out, torch.int32, n), p, s, d, a, part.data_ptr())
+
+    def evict(self, kvk, kvv, score, kept, pos_out, pos, part, budget: int, n_sink: int = 0, n_recent: int = 0, kslot=None,
+              kslot_dst=None, act=None):
+        """Keeps `budget` of the pos[i] cached positions of every sequence: the first n_sink, the last n_recent and the best
+        scored between them, moved to the front of the same partition or of kslot_dst[i]'s."""
+        k, v = self._cache_ptrs(kvk, kvv, False, kslot is not None)
+        g = self.geom
+        n, args = self._evict_args(score, kept, pos_out, pos, part, budget, kslot, kslot_dst, act,
+                                   (1 if kslot is None else g.n_slots) * g.n_kv * g.slot_ctx)
+        self._check("battn_evict", self.lib.battn_evict(self.h, k, v, *args, budget, n_sink, n_recent, n, self._stream_here()))
+
+    def evict_paged(self, pages, score, kept, pos_out, pos, part, budget: int, n_sink: int = 0, n_recent: int = 0, ktab=None,
+                    ktab_dst=None, act=None):
+        n, args = self._evict_args(score, kept, pos_out, pos, part, budget, ktab, ktab_dst, act,
+                                   (1 if ktab is None else pages.n_tables) * self.geom.n_kv * pages.max_pages * pages.page_len)
+        self._check("battn_evict_paged", self.lib.battn_evict_paged(self.h, C.byref(pages), *args, budget, n_sink, n_recent, n,
+                                                                    self._stream_here()))
+
     # ---- the step after attention ------------------------------------------------------------------------
     def gate_norm(self, dst, aout, gate, sgate, xq, xd, xsum, rows: int):
         """k_gate_norm_vec4 (bruce.cu:1526): sigmoid gate, L2 norm, q8 activation copy; dst may be None."""

@@ -378,6 +378,35 @@ int battn_attend_sinks(battn_handle* h, void* out, const void* q, const uint8_t*
 int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const battn_pages* pages, const battn_sinks* sinks,
                              const int* pos, const int* ktab, const int* act, void* ws, int rows, int n_seq, void* stream);
 
+/* ---- Eviction by accumulated attention weight ----------------------------------------------------------------------
+ * (No counterpart in the reference, whose full layers hold every position of a conversation.)  Trims a full-causal layer
+ * to `budget` positions per sequence.  `score`, fp32 [slot][kv head][slot_ctx] (paged: [table row][kv head][max_pages *
+ * page_len]), is what battn_attend_track accumulated; any other measure will do.  Of a sequence that holds
+ * n = pos[i] > budget positions every kv head keeps, each by its own scores,
+ *     the first n_sink, the last n_recent, and of the rest the budget - n_sink - n_recent best scored
+ * (equal scores: the lower position stays; NaN counts as the lowest score, -0 as 0), in their order.  Their records and
+ * scores move to positions 0 .. budget-1, so that the next token goes to position `budget` and "recent" keeps its meaning;
+ * records carry the rotation they were stored with, so hosts count rotary positions apart from cache positions.  With
+ * n <= budget everything stays.
+ *   kept     [n_seq][kv head][budget]: the position each record came from, ascending; -1 past min(n, budget)
+ *   pos_out  [n_seq]: min(n, budget); may be pos itself
+ *   kslot_dst  NULL: in place.  Otherwise the partition (or table row) that receives sequence i, which another sequence of
+ *              the call must neither read nor write (a clash sets BATTN_DEV_BAD_POSITION and skips it); the source
+ *              keeps its records and scores.  So a conversation can be trimmed out of a prompt that others share.
+ *   paged      the pages behind the first min(n, budget) positions of the target row must be mapped, and in place not
+ *              shared with another sequence (un-share them first, as before an append); pages past them are free
+ *              afterwards.  Two rows of one call may share source pages; a target page is in no other place of the call.
+ *   ws         battn_evict_workspace_bytes(n_seq)
+ * Sequences with act[i] == 0 or a bad position or slot are left alone, their kept and pos_out too.  The result does not
+ * depend on timing: no floating-point sum is formed, and records are copied. */
+int battn_evict_workspace_bytes(const battn_handle* h, int n_seq, size_t* out_bytes);
+int battn_evict(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score, int* kept, int* pos_out, const int* pos,
+                const int* kslot, const int* kslot_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
+                int n_seq, void* stream);
+int battn_evict_paged(battn_handle* h, const battn_pages* pages, float* score, int* kept, int* pos_out, const int* pos,
+                      const int* ktab, const int* ktab_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
+                      int n_seq, void* stream);
+
 /* ---- One sequence split by position range across several devices (no counterpart in the reference, which is
  * single-GPU; built on its split record and merge, bruce.cu:781-783, 992-1007) ------------------------------------
  * Device r of `world` holds positions [r*N/world, (r+1)*N/world) of the sequence in its own cache, with LOCAL

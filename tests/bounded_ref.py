@@ -138,3 +138,15 @@ def put(eng, buf, recs, is_swa: bool, which: int):
 
 def ids(x, eng):
     return dev_i32(x, eng.device)
+
+
+def evict_list(score: np.ndarray, budget: int, n_sink: int, n_recent: int) -> np.ndarray:
+    """Positions of one kv head that stay of len(score), ascending: NaN lowest, ties to the lower position."""
+    n = len(score)
+    if n <= budget:
+        return np.arange(n)
+    mid = np.arange(n_sink, n - n_recent)
+    s = score[mid].astype(np.float64)
+    order = np.lexsort((mid, np.where(np.isnan(s), 0.0, -s), np.isnan(s)))        # not NaN first, then best, then lowest
+    keep = mid[order[:budget - n_sink - n_recent]]
+    return np.concatenate([np.arange(n_sink), np.sort(keep), np.arange(n - n_recent, n)])
