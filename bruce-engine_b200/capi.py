@@ -10,7 +10,7 @@ LIB_PATH = os.path.join(HERE, "libbattn.so")
 
 IPC_HANDLE_BYTES = 64
 OK, ERR_ARG, ERR_CAPACITY, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3, 4
-DEV_BAD_POSITION, DEV_WAIT_TIMEOUT = 1, 2
+DEV_BAD_POSITION, DEV_WAIT_TIMEOUT, DEV_WORKSPACE = 1, 2, 4
 STATUS_NAMES = {0: "BATTN_OK", 1: "BATTN_ERR_ARG", 2: "BATTN_ERR_CAPACITY", 3: "BATTN_ERR_CUDA",
                 4: "BATTN_ERR_DEVICE"}
 
@@ -81,6 +81,9 @@ SIGNATURES = {
     "battn_sinks_store": (_I, [_P, _P, _P, _SK] + [_P] * 3 + [_I, _I, _P]),
     "battn_attend_sinks": (_I, [_P] * 5 + [_SK] + [_P] * 4 + [_I, _I, _I, _P]),
     "battn_attend_sinks_paged": (_I, [_P] * 3 + [_PG, _SK] + [_P] * 4 + [_I, _I, _P]),
+    "battn_track_workspace_bytes": (_I, [_P, _I, _I, C.c_longlong, _SZP]),
+    "battn_attend_track": (_I, [_P] * 11 + [C.c_size_t, _I, _I, _P]),
+    "battn_attend_track_paged": (_I, [_P] * 5 + [_PG] + [_P] * 4 + [C.c_size_t, _I, _I, _P]),
     "battn_evict_workspace_bytes": (_I, [_P, _I, _SZP]),
     "battn_evict": (_I, [_P] * 11 + [_I] * 4 + [_P]),
     "battn_evict_paged": (_I, [_P, _PG] + [_P] * 8 + [_I] * 4 + [_P]),

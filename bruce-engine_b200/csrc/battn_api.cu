@@ -16,6 +16,7 @@
 #include "prefill.cuh"
 #include "prefill_hd128.cuh"
 #include "sinks.cuh"
+#include "track.cuh"
 #include "verify.cuh"
 #include "verify_tc.cuh"
 
@@ -95,9 +96,18 @@ cudaError_t fd_prepare_all(battn_handle* h) {
         if ((e = allow_smem(vt::k_verify_tc<VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
         if ((e = allow_smem(pf128::k_prefill_hd128<false, VAR_SINK>, pf128::TOTAL)) != cudaSuccess) return e;
         if ((e = allow_smem(pf128::k_prefill_hd128<true, VAR_SINK>, pf128::TOTAL_PAIR)) != cudaSuccess) return e;
+        if ((e = allow_smem(pf128::k_prefill_hd128<false, VAR_TRACK>, pf128::TOTAL)) != cudaSuccess) return e;
+        if ((e = allow_smem(pf128::k_prefill_hd128<true, VAR_TRACK>, pf128::TOTAL_PAIR)) != cudaSuccess) return e;
     } else {
         if ((e = allow_smem(pf::k_prefill<256, 64, VAR_SINK>, pf::Cfg<256, 64>::TOTAL)) != cudaSuccess) return e;
+        if ((e = allow_smem(pf::k_prefill<256, 64, VAR_TRACK>, pf::Cfg<256, 64>::TOTAL)) != cudaSuccess) return e;
     }
+    if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_TRACK>, SMEM_MAX)) != cudaSuccess) return e;
+    if ((e = allow_smem(tr::k_track_chunk<HD>, tr::ChunkCfg<HD>::SMEM)) != cudaSuccess) return e;
+    h->track_ctas_per_sm = 1;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&h->track_ctas_per_sm, (const void*)tr::k_track_chunk<HD>, tr::CTHREADS,
+                                                      tr::ChunkCfg<HD>::SMEM);
+    if (e != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_select, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::SMEM)) != cudaSuccess) return e;
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
@@ -270,8 +280,20 @@ struct PrologueIn {
     int table_off;
 };
 
+// what a variant of the decode / verify call adds
+struct StepVariant {
+    int var;
+    SinkView sink;               // VAR_SINK
+    float* scores;               // VAR_TRACK, see fd::Params
+    int sc_tiles;
+    int cph;                     // out, VAR_TRACK: the work cut the call took
+};
+
 template <int HD, int NT>
 cudaError_t launch_fd_kernel(const fd::Params& P, int grid, size_t smem, cudaStream_t st, int var) {
+    if constexpr (NT == 1) {
+        if (var == VAR_TRACK) return launch_pdl(fd::k_flash_decode<HD, 1, 0, VAR_TRACK>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
+    }
     if (var == VAR_SINK) return launch_pdl(fd::k_flash_decode<HD, NT, 0, VAR_SINK>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
     if constexpr (NT == 1) {
         if (P.q_raw) return launch_pdl(fd::k_flash_decode<HD, 1, 2>, dim3(grid), dim3(fd::NTHREADS), smem, st, P);
@@ -285,9 +307,10 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
                  const int* pos, const int* kslot, const int* act, void* ws, int n_seq, int rows, int is_swa,
                  cudaStream_t st, const XchgView* xv = nullptr, int* epoch_ptr = nullptr, int epoch_advance = 0,
                  const PagedView* pv = nullptr, const float* k_new = nullptr, const float* v_new = nullptr,
-                 const PrologueIn* pro = nullptr, const SinkView* sink = nullptr) {
+                 const PrologueIn* pro = nullptr, StepVariant* sv = nullptr) {
     const Geom& g = h->g;
-    const int var = sink ? VAR_SINK : VAR_PLAIN;
+    const int var = sv ? sv->var : VAR_PLAIN;
+    const bool sink = var == VAR_SINK;
     const int RG = rows * g.G;
     if (RG > 32) return BATTN_ERR_CAPACITY;
     const int idx = nt_index(RG);
@@ -302,7 +325,7 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
     P.epoch_ptr = epoch_ptr; P.epoch_advance = epoch_advance;
     P.cph = 0;
-    if (sink) P.sink = *sink;
+    if (sv) { P.sink = sv->sink; P.scores = sv->scores; P.sc_tiles = sv->sc_tiles; }
     P.q_raw = pro ? pro->q_raw : nullptr; P.sqk = pro ? pro->sqk : nullptr; P.cs = pro ? pro->cs : nullptr;
     P.sn = pro ? pro->sn : nullptr; P.table_off = pro ? pro->table_off : 0;
     P.k_new = k_new; P.v_new = v_new; P.kvk_w = const_cast<uint8_t*>(kvk); P.kvv_w = const_cast<uint8_t*>(kvv);
@@ -358,6 +381,7 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     M.n_rows = n_seq * rows; M.rows = rows; M.Hq = g.Hq; M.Hkv = g.Hkv; M.G = g.G;
     M.count = 0; M.log2_domain = 1; M.out_f16 = g.out_f16; M.hdr = P.hdr; M.status = h->d_status;
     M.cph = P.cph;
+    if (sv) sv->cph = P.cph;
     if (P.early && fd_grid > 0 && n_seq == 1 && var == VAR_PLAIN) {
         // the merge recomputes the cut from the positions while it waits for the decode kernel
         M.pre_grid = fd_grid; M.pre_tile = fd::TILE;
@@ -377,6 +401,8 @@ struct ChunkVariant {
     const int* kslot;
     const int* act;
     SinkView sink;               // VAR_SINK
+    float2* stats;               // VAR_TRACK, see pf::Params
+    float* lse;
 };
 
 // prompt chunk on the tcgen05 kernel: one CTA per (128-row M tile, kv head), normalised output
@@ -396,6 +422,7 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
     const int var = cv ? cv->var : VAR_PLAIN;
     if (cv) {
         P.kslot = cv->kslot; P.act = cv->act; P.n_slots = pv ? pv->n_tables : g.n_slots; P.sink = cv->sink;
+        P.stats = cv->stats; P.lse = cv->lse;
     }
     // early KV streaming: only behind the append / prologue of exactly this chunk, or no cache write
     P.early = h->early_stream &&
@@ -419,11 +446,17 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
             attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
             attr[1].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr; cfg.numAttrs = 2;
-            cudaLaunchKernelEx(&cfg, var == VAR_SINK ? pf128::k_prefill_hd128<true, VAR_SINK> : pf128::k_prefill_hd128<true>, P);
+            cudaLaunchKernelEx(&cfg, var == VAR_SINK    ? pf128::k_prefill_hd128<true, VAR_SINK>
+                                     : var == VAR_TRACK ? pf128::k_prefill_hd128<true, VAR_TRACK>
+                                                        : pf128::k_prefill_hd128<true>, P);
         } else if (g.HD == 128) {
-            launch_pdl(var == VAR_SINK ? pf128::k_prefill_hd128<false, VAR_SINK> : pf128::k_prefill_hd128<false>, grid, dim3(pf128::NTHREADS), pf128::TOTAL, st, P);
+            launch_pdl(var == VAR_SINK    ? pf128::k_prefill_hd128<false, VAR_SINK>
+                       : var == VAR_TRACK ? pf128::k_prefill_hd128<false, VAR_TRACK>
+                                          : pf128::k_prefill_hd128<false>, grid, dim3(pf128::NTHREADS), pf128::TOTAL, st, P);
         }
-        else             launch_pdl(var == VAR_SINK ? pf::k_prefill<256, 64, VAR_SINK> : pf::k_prefill<256, 64>, grid, dim3(pf::NTHREADS), pf::Cfg<256, 64>::TOTAL, st, P);
+        else             launch_pdl(var == VAR_SINK    ? pf::k_prefill<256, 64, VAR_SINK>
+                                    : var == VAR_TRACK ? pf::k_prefill<256, 64, VAR_TRACK>
+                                                       : pf::k_prefill<256, 64>, grid, dim3(pf::NTHREADS), pf::Cfg<256, 64>::TOTAL, st, P);
     }
     h->launches += 1;
     cudaError_t e = cudaGetLastError();
@@ -445,6 +478,7 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
         if (cv) {                                // an idle sequence left no records
             M.pos = pos; M.kslot = cv->kslot; M.act = cv->act; M.is_swa = is_swa; M.W = g.W; M.slot_ctx = P.slot_ctx;
             M.n_slots = P.n_slots;
+            M.stats = cv->stats; M.lse = cv->lse;
         }
         // (head_dim 128: programmatic launch, the merge's blocks are resident and past their launch when the prompt
         // kernel drains -- 2 us less on a short chunk; at head_dim 256, where every 512-row chunk is split and the merge
@@ -966,13 +1000,15 @@ static int attend_sinks_impl(battn_handle* h, void* out, const void* q, const ui
     if (rc) return rc;
     if (!ws || ((uintptr_t)ws & 15)) return BATTN_ERR_ARG;
     const Geom& g = h->g;
-    ChunkVariant cv{VAR_SINK, kslot, act, {}};
+    ChunkVariant cv{VAR_SINK, kslot, act, {}, nullptr, nullptr};
     if ((rc = sink_view(g, sinks, is_swa, cv.sink))) return rc;
     const DeviceScope dev(h->device);
     cudaStream_t st = (cudaStream_t)stream;
-    if (rows <= MAX_VERIFY && rows * g.G <= 32)
+    if (rows <= MAX_VERIFY && rows * g.G <= 32) {
+        StepVariant sv{VAR_SINK, cv.sink, nullptr, 0, 0};
         return launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, rows, is_swa, st, nullptr, nullptr, 0, pv,
-                            nullptr, nullptr, nullptr, &cv.sink);
+                            nullptr, nullptr, nullptr, &sv);
+    }
     // a prompt chunk: one sequence, and the bounds of battn_prefill
     if (n_seq != 1 || (is_swa && rows > g.W)) return BATTN_ERR_CAPACITY;
     if (g.W < 64) return BATTN_ERR_ARG;
@@ -991,6 +1027,95 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
     const int rc = paged_view(pages, pv);
     if (rc) return rc;
     return attend_sinks_impl(h, out, q, pages->pool_k, pages->pool_v, sinks, pos, ktab, act, ws, rows, n_seq, 0, stream, &pv);
+}
+
+// ---- attention that accumulates its weights -----------------------------------------------------------------------
+// scratch of a prompt chunk: split records, their statistics, the rows' log-sum-exps
+struct TrackChunkWs {
+    size_t stats, lse, total;
+};
+static TrackChunkWs track_chunk_workspace(const battn_handle* h, int rows) {
+    const size_t per = (size_t)rows * h->g.Hq;
+    TrackChunkWs w;
+    w.stats = align_up(prefill_workspace(h, rows), 256);
+    w.lse = w.stats + align_up(per * prefill_splits(h, rows, 0) * sizeof(float2), 256);
+    w.total = w.lse + align_up(per * sizeof(float), 256);
+    return w;
+}
+
+int battn_track_workspace_bytes(const battn_handle* h, int n_seq, int rows_per_seq, long long max_positions, size_t* out_bytes) {
+    if (!h || !out_bytes || n_seq < 1 || rows_per_seq < 1 || max_positions < 0) return BATTN_ERR_ARG;
+    if (n_seq > MAX_SEQ || rows_per_seq > MAX_PREFILL) return BATTN_ERR_CAPACITY;
+    const Geom& g = h->g;
+    const size_t tiles = (size_t)g.Hkv * ((size_t)(max_positions / fd::TILE) + n_seq);
+    size_t need = align_up(fd_workspace(h, n_seq, 1).total, 256) + tiles * fd::TILE * g.G * sizeof(float);
+    for (int r = 2; r <= rows_per_seq; ++r) need = std::max(need, track_chunk_workspace(h, r).total);
+    *out_bytes = align_up(need, 256);
+    return BATTN_OK;
+}
+
+static int attend_track_impl(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q,
+                             const uint8_t* kvk, const uint8_t* kvv, const int* pos, const int* kslot, const int* act, void* ws,
+                             size_t ws_bytes, int rows, int n_seq, void* stream, const PagedView* pv) {
+    int rc = check_seq_args(h, out, q, kvk, kvv, pos, kslot, n_seq, rows, MAX_PREFILL);
+    if (rc) return rc;
+    if (!ws || ((uintptr_t)ws & 15) || !score_out || (((uintptr_t)score_out | (uintptr_t)score_in) & 15)) return BATTN_ERR_ARG;
+    const Geom& g = h->g;
+    const DeviceScope dev(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    uint8_t* w = reinterpret_cast<uint8_t*>(ws);
+    cudaError_t e;
+    if (rows == 1) {
+        const size_t base = align_up(fd_workspace(h, n_seq, 1).total, 256), tile = (size_t)fd::TILE * g.G * sizeof(float);
+        if (ws_bytes < base + tile) return BATTN_ERR_CAPACITY;
+        const size_t tiles = (ws_bytes - base) / tile;
+        StepVariant sv{VAR_TRACK, {}, reinterpret_cast<float*>(w + base), (int)std::min<size_t>(tiles, 0x7fffffff), 0};
+        rc = launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, 1, 0, st, nullptr, nullptr, 0, pv, nullptr,
+                          nullptr, nullptr, &sv);
+        if (rc) return rc;
+        const FdWs fw = fd_workspace(h, n_seq, 1);
+        tr::StepParams P;
+        P.hdr = reinterpret_cast<const int*>(ws); P.part = reinterpret_cast<const float*>(w + fw.hdr_bytes);
+        P.scores = sv.scores; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot;
+        P.n_seq = n_seq; P.Hkv = g.Hkv; P.G = g.G; P.HD = g.HD; P.cph = sv.cph;
+        P.stride = pv ? (size_t)pv->capacity : (size_t)g.slot_ctx;
+        e = launch_pdl(tr::k_track_step, dim3(h->num_sms * 2), dim3(tr::STEP_THREADS), (n_seq + 1) * sizeof(int), st, P);
+    } else {
+        if (n_seq != 1) return BATTN_ERR_CAPACITY;
+        const TrackChunkWs cw = track_chunk_workspace(h, rows);
+        if (ws_bytes < cw.total) return BATTN_ERR_CAPACITY;
+        if (g.W < 64) return BATTN_ERR_ARG;                     // as battn_prefill
+        ChunkVariant cv{VAR_TRACK, kslot, act, {}, reinterpret_cast<float2*>(w + cw.stats), reinterpret_cast<float*>(w + cw.lse)};
+        if ((rc = launch_prefill(h, out, q, kvk, kvv, pos, ws, rows, 0, st, nullptr, pv, 0, &cv))) return rc;
+        tr::ChunkParams P;
+        P.q = q; P.kvk = kvk; P.lse = cv.lse; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot; P.act = act;
+        P.rows = rows; P.Hq = g.Hq; P.Hkv = g.Hkv; P.G = g.G; P.q_f16 = g.q_f16;
+        P.pstride = pv ? pv->capacity : g.slot_ctx; P.n_slots = pv ? pv->n_tables : g.n_slots;
+        P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
+        if (pv) P.pg = pv->pg;
+        const dim3 grid(h->num_sms * std::max(1, h->track_ctas_per_sm)), block(tr::CTHREADS);
+        e = g.HD == 128 ? launch_pdl(tr::k_track_chunk<128>, grid, block, tr::ChunkCfg<128>::SMEM, st, P)
+                        : launch_pdl(tr::k_track_chunk<256>, grid, block, tr::ChunkCfg<256>::SMEM, st, P);
+    }
+    h->launches += 1;
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? BATTN_OK : cuda_fail(h, e);
+}
+
+int battn_attend_track(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q, const uint8_t* kvk,
+                       const uint8_t* kvv, const int* pos, const int* kslot, const int* act, void* ws, size_t ws_bytes, int rows,
+                       int n_seq, void* stream) {
+    return attend_track_impl(h, out, score_out, score_in, q, kvk, kvv, pos, kslot, act, ws, ws_bytes, rows, n_seq, stream, nullptr);
+}
+
+int battn_attend_track_paged(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q,
+                             const battn_pages* pages, const int* pos, const int* ktab, const int* act, void* ws, size_t ws_bytes,
+                             int rows, int n_seq, void* stream) {
+    PagedView pv;
+    const int rc = paged_view(pages, pv);
+    if (rc) return rc;
+    return attend_track_impl(h, out, score_out, score_in, q, pages->pool_k, pages->pool_v, pos, ktab, act, ws, ws_bytes, rows,
+                             n_seq, stream, &pv);
 }
 
 // ---- eviction by accumulated attention weight ------------------------------------------------------------------

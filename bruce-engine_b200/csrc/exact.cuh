@@ -214,6 +214,10 @@ struct MergeParams {
     // positions before the wait (pre_grid CTAs, pre_tile keys per tile) instead of read from the header after it
     int pre_grid, pre_tile;
     int cph;               // the decode kernel's cut: > 0: one sequence, cph CTAs per kv head; 0: linear
+    // GATHERED behind a weight-accumulating prompt chunk: its splits' statistics [split][row][head] = (m, l) in log2 units,
+    // joined into lse [row][head] = m + log2(l)
+    const float2* stats;
+    float* lse;
     // sequence split across devices (k_merge_balanced as the pushing epilogue, k_merge_wait): see XchgView
     XchgView xchg;
 };
@@ -256,6 +260,17 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_merge(const MergeParams P) {
     }
     count = min(count, MERGE_MAX_COUNT);
 
+    if (P.stats && warp == 0) {
+        const size_t si = (size_t)rowidx * P.Hq + hq, step = (size_t)P.n_rows * P.Hq;
+        float2 st = lane < count ? P.stats[si + lane * step] : make_float2(NEG_BIG, 0.f);       // at most 8 splits
+        float M = st.x;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float L = st.y * fast_exp2(st.x - M);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane == 0) P.lse[si] = M + log2f(L);
+    }
     // phase 1: (m, l) of every record, block max of m
     float mx = NEG_BIG;
     for (int s = tid; s < count; s += MERGE_THREADS) {

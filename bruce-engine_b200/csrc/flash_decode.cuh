@@ -84,6 +84,10 @@ struct Params {
     uint8_t* kvk_w;  // the caches again, writable
     uint8_t* kvv_w;
     SinkView sink;   // VAR_SINK
+    // VAR_TRACK (one row per sequence): the scores of every visible key, log2 units, [global tile][key][head of the group];
+    // room for sc_tiles tiles.  A call that needs more sets BATTN_DEV_WORKSPACE and does nothing.
+    float* scores;
+    int sc_tiles;
 };
 
 template <int HD>
@@ -106,7 +110,7 @@ __device__ __forceinline__ int perm16(int kappa) { return kappa ^ ((kappa >> 2) 
 
 // AP: 1 = the decode call that appends its own (prepared) row, 2 = the one that also runs the QKV prologue of its row
 // (separate instances, so that the plain kernel carries none of it)
-// VAR: VAR_SINK = sliding window with sinks
+// VAR: VAR_SINK = sliding window with sinks, VAR_TRACK = the scores are kept for the weights (track.cuh)
 template <int HD, int NT, int AP = 0, int VAR = VAR_PLAIN>
 __global__ void __launch_bounds__(NTHREADS, (NT == 1 ? 3 : (NT == 2 ? 2 : 1)))
 k_flash_decode(const Params P) {
@@ -115,6 +119,7 @@ k_flash_decode(const Params P) {
     constexpr int STAGES = stages_of<HD, NT>();
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_abort;
+    __shared__ float s_lx[VAR == VAR_TRACK ? NW * 8 : 1];        // VAR_TRACK: the warps' unrounded denominators
     const int RG = P.RG;
     uint8_t* stages = smem;
     __half* qs = reinterpret_cast<__half*>(smem + STAGES * 2 * TILE_BYTES);
@@ -171,6 +176,14 @@ k_flash_decode(const Params P) {
     const int total = P.Hkv * cum[P.n_seq];
     const Share share = cut_share(cum, P.n_seq, P.Hkv, P.cph, (int)blockIdx.x, (int)gridDim.x);
     const int per = share.per;
+    if (VAR == VAR_TRACK && total > P.sc_tiles) {                    // every CTA alike: the merge finds nothing to do
+        if (early) { pdl_wait(); pdl_trigger(); }
+        if (blockIdx.x == 0) {
+            if (tid == 0) { atomicOr(P.status, BATTN_DEV_WORKSPACE); P.hdr[0] = 1; P.hdr[1] = 0; }
+            for (int i = tid; i <= P.n_seq; i += NTHREADS) P.hdr[2 + i] = 0;
+        }
+        return;
+    }
     if (blockIdx.x == 0) {
         // the header and the step counter are read by the previous call's merge: written after the wait
         if (early) { pdl_wait(); pdl_trigger(); }
@@ -311,6 +324,7 @@ k_flash_decode(const Params P) {
             const int full_lo = VAR == VAR_SINK || P.is_swa ? max(0, sr.p0 + P.rows - P.W) : 0;      // window start of the last row
 
             float m[NT][2], l[NT][2], O[NBLK][2][NT][4];
+            float lx[VAR == VAR_TRACK ? 2 : 1] = {};                              // as l, of the unrounded weights
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 m[nt][0] = m[nt][1] = NEG_BIG;
@@ -434,6 +448,7 @@ k_flash_decode(const Params P) {
                             if (key0 > lim[nt][e] || below_window<VAR>(key0, low[nt][e], P.sink)) v0 = NEG_BIG;
                             if (key1 > lim[nt][e] || below_window<VAR>(key1, low[nt][e], P.sink)) v1 = NEG_BIG;
                         }
+                        if constexpr (VAR == VAR_TRACK) { sv[nt][e] = v0; sv[nt][2 + e] = v1; }
                         float mx = fmaxf(v0, v1);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
@@ -445,6 +460,7 @@ k_flash_decode(const Params P) {
                             if (v0 < -1e29f) p0 = 0.f;
                             if (v1 < -1e29f) p1 = 0.f;
                         }
+                        if constexpr (VAR == VAR_TRACK) lx[e] = fmaf(lx[e], al, p0 + p1);
                         any_rescale |= (mn != m[nt][e]);
                         alpha[nt][e] = al;
                         m[nt][e] = mn;
@@ -459,6 +475,20 @@ k_flash_decode(const Params P) {
                     l[nt][1] = fmaf(l[nt][1], alpha[nt][1], f01.y + f23.y);
                     pb0[nt] = movmatrix_trans(h01);     // keys kappa = 2t4, 2t4+1
                     pb1[nt] = movmatrix_trans(h23);     // keys kappa = 2t4+8, 2t4+9
+                }
+                if constexpr (VAR == VAR_TRACK) {
+                    // columns 2 t4, 2 t4 + 1 are heads of the group (one row): 16 bytes per key at four heads
+                    float* sc = P.scores + (size_t)(g + t) * (TILE * P.G);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float* at = sc + (k ? kl1 : kl0) * P.G + 2 * t4;
+                        if (!(P.G & 1)) {
+                            if (2 * t4 < P.G) *reinterpret_cast<float2*>(at) = make_float2(sv[0][2 * k], sv[0][2 * k + 1]);
+                        } else {
+                            if (2 * t4 < P.G) at[0] = sv[0][2 * k];
+                            if (2 * t4 + 1 < P.G) at[1] = sv[0][2 * k + 1];
+                        }
+                    }
                 }
                 if (__any_sync(0xffffffffu, any_rescale)) {
 #pragma unroll
@@ -549,6 +579,16 @@ k_flash_decode(const Params P) {
                     v += __shfl_xor_sync(0xffffffffu, v, 16);
                     l[nt][e] = v;
                 }
+            if constexpr (VAR == VAR_TRACK) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v = lx[e];
+                    v += __shfl_xor_sync(0xffffffffu, v, 4);
+                    v += __shfl_xor_sync(0xffffffffu, v, 8);
+                    v += __shfl_xor_sync(0xffffffffu, v, 16);
+                    if (gid == 0) s_lx[warp * 8 + 2 * t4 + e] = v;
+                }
+            }
             float* mb = mbuf + (size_t)warp * RG * (HD + 2);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -587,6 +627,12 @@ k_flash_decode(const Params P) {
                 }
                 dst[(size_t)n * (HD + 4) + d] = acc;
                 if (d == 0) { dst[(size_t)n * (HD + 4) + HD] = M; dst[(size_t)n * (HD + 4) + HD + 1] = L; }
+                if (VAR == VAR_TRACK && d == 0) {              // in the record's padding
+                    float lsum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) lsum = fmaf(s_lx[w * 8 + n], fast_exp2(mw[w] - M), lsum);
+                    dst[(size_t)n * (HD + 4) + HD + 2] = lsum;
+                }
             }
             g += pc.n;
         }

@@ -325,6 +325,37 @@ class AttnEngine:
             self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), C.byref(pages),
             C.byref(sinks), p, s, a, part.data_ptr(), rows, n, self._stream_here()))
 
+    # ---- attention that accumulates its weights ------------------------------------------------------------
+    def alloc_track_part(self, n_seq: int, rows: int, max_positions: int) -> torch.Tensor:
+        n = C.c_size_t()
+        self._check("battn_track_workspace_bytes",
+                    self.lib.battn_track_workspace_bytes(self.h, n_seq, rows, max_positions, C.byref(n)))
+        return torch.empty(n.value, dtype=torch.uint8, device=self.device)
+
+    def _track_args(self, out, score_out, score_in, q, rows, n, scores):
+        nq = n * rows * self.geom.n_head * self.geom.head_dim
+        return (self._dev("out", out, self.out_torch, nq), self._dev("score_out", score_out, torch.float32, scores),
+                None if score_in is None else self._dev("score_in", score_in, torch.float32, scores),
+                self._dev("q", q, self.q_torch, nq))
+
+    def attn_track(self, out, score_out, score_in, q, kvk, kvv, pos, part, rows: int = 1, kslot=None, act=None):
+        """Full-causal attention (one row of every sequence, or 2..512 rows of one) that also adds the weight every cached
+        position receives to score_in, into score_out (the same tensor, usually); score_in None: nothing so far."""
+        g = self.geom
+        p, s, a, n = self._seqs(pos, kslot, act)
+        k, v = self._cache_ptrs(kvk, kvv, False, kslot is not None)
+        args = self._track_args(out, score_out, score_in, q, rows, n, (1 if kslot is None else g.n_slots) * g.n_kv * g.slot_ctx)
+        self._check("battn_attend_track", self.lib.battn_attend_track(
+            self.h, *args, k, v, p, s, a, part.data_ptr(), part.numel() * part.element_size(), rows, n, self._stream_here()))
+
+    def attn_track_paged(self, out, score_out, score_in, q, pages, pos, part, rows: int = 1, ktab=None, act=None):
+        p, s, a, n = self._seqs(pos, ktab, act)
+        args = self._track_args(out, score_out, score_in, q, rows, n, (1 if ktab is None else pages.n_tables) *
+                                self.geom.n_kv * pages.max_pages * pages.page_len)
+        self._check("battn_attend_track_paged", self.lib.battn_attend_track_paged(
+            self.h, *args, C.byref(pages), p, s, a, part.data_ptr(), part.numel() * part.element_size(), rows, n,
+            self._stream_here()))
+
     # ---- eviction by accumulated attention weight --------------------------------------------------------
     def alloc_evict_part(self, n_seq: int) -> torch.Tensor:
         n = C.c_size_t()

@@ -55,7 +55,8 @@ enum { BATTN_F32 = 0, BATTN_F16 = 1 };
 /* bits of the device status word (battn_device_status) */
 enum {
     BATTN_DEV_BAD_POSITION = 1,  /* a row's position fell outside the cache; the row was skipped  */
-    BATTN_DEV_WAIT_TIMEOUT = 2   /* a bounded in-kernel wait ran out; results of that launch void */
+    BATTN_DEV_WAIT_TIMEOUT = 2,  /* a bounded in-kernel wait ran out; results of that launch void */
+    BATTN_DEV_WORKSPACE    = 4   /* battn_attend_track: more cached positions than ws has room for; call skipped */
 };
 
 /* Geometry: the reference fixes these with #defines (bruce.cu:43-53); here they are run-time. */
@@ -377,6 +378,31 @@ int battn_attend_sinks(battn_handle* h, void* out, const void* q, const uint8_t*
                        int n_seq, int is_swa, void* stream);
 int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const battn_pages* pages, const battn_sinks* sinks,
                              const int* pos, const int* ktab, const int* act, void* ws, int rows, int n_seq, void* stream);
+
+/* ---- Attention that accumulates its weights ---------------------------------------------------------------------------
+ * (No counterpart in the reference.)  Attention over a full-causal layer that also adds up, for every cached position and
+ * kv head, the softmax weight the position received from the call's rows and the query heads of the kv head's group:
+ *     out as battn_decode / battn_prefill,
+ *     score_out[kv head][p] = (p < pos[i] ? score_in[kv head][p] : 0) + sum over rows r and heads h of w[r][h][p]
+ * for p <= pos[i]+rows-1; positions past them are not touched, and the call's own positions start from nothing, so the
+ * buffers need no clearing when a slot begins a new sequence.  score_in == NULL: nothing was accumulated before (the last
+ * rows of a prompt choose what is kept of it).  score_in may be score_out, but not overlap it otherwise.
+ *   score_*  fp32 [slot][kv head][slot_ctx] (paged: [table row][kv head][max_pages * page_len]); with kslot == NULL the
+ *            slot's own [kv head][slot_ctx]; 16-byte aligned
+ *   rows     1: n_seq sequences, one new token each.  2 .. 512: a prompt chunk, or the accepted rows of a speculative
+ *            round, of one sequence (n_seq = 1); group a divisor of 128, window >= 64, as battn_prefill
+ *   ws       battn_track_workspace_bytes bytes (ws_bytes says how many it has).  The one-row call keeps the scores of every
+ *            position there: max_positions bounds the sum over the active sequences of the positions they hold, the new ones
+ *            included.  A call that meets more sets BATTN_DEV_WORKSPACE and writes nothing.
+ * The weights divide by a denominator that is summed in fp32 from unrounded weights (the output divides by the sum of the
+ * fp16 weights its product uses); fp32 queries are rounded to fp16 first, as everywhere.  No atomics: results repeat. */
+int battn_track_workspace_bytes(const battn_handle* h, int n_seq, int rows_per_seq, long long max_positions, size_t* out_bytes);
+int battn_attend_track(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q, const uint8_t* kvk,
+                       const uint8_t* kvv, const int* pos, const int* kslot, const int* act, void* ws, size_t ws_bytes, int rows,
+                       int n_seq, void* stream);
+int battn_attend_track_paged(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q,
+                             const battn_pages* pages, const int* pos, const int* ktab, const int* act, void* ws, size_t ws_bytes,
+                             int rows, int n_seq, void* stream);
 
 /* ---- Eviction by accumulated attention weight ----------------------------------------------------------------------
  * (No counterpart in the reference, whose full layers hold every position of a conversation.)  Trims a full-causal layer

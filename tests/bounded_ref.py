@@ -150,3 +150,29 @@ def evict_list(score: np.ndarray, budget: int, n_sink: int, n_recent: int) -> np
     order = np.lexsort((mid, np.where(np.isnan(s), 0.0, -s), np.isnan(s)))        # not NaN first, then best, then lowest
     keep = mid[order[:budget - n_sink - n_recent]]
     return np.concatenate([np.arange(n_sink), np.sort(keep), np.arange(n - n_recent, n)])
+
+
+def score64(g, q, krec, p0: int, score_in):
+    """Accumulated weights [n_kv][p0 + rows] in float64."""
+    s = weights64(g, q, krec, p0).sum(1).reshape(g.n_kv, g.group, -1).sum(1)
+    if score_in is not None:
+        s[:, :p0] += score_in[:, :p0]
+    return s
+
+
+def assert_scores(got, want, g, q, krec, p0, what=""):
+    """Accumulated weights against 64 bits.
+
+    A weight is 2^(s - lse).  s is a sum of exact products in fp32 (blocks of 32 dims, then at most 8 scaled blocks): off by
+    less than 16 * 2^-23 of A = sum |q_d k_d| * scale * log2(e), and so is lse, a convex mean of such errors; 2^x turns a
+    difference d of exponents into a factor 1 + d ln 2.  The denominator adds n / 2 terms or fewer in a row, a position's
+    weight at most rows * group: each addition is off by 2^-24 of a sum of positive terms.  ex2.approx is off by 2^-22, twice
+    per weight and once per merge level: 8 * 2^-22.  The accumulated value adds one rounding."""
+    n = krec.shape[1]
+    kd = np.abs(values(krec, g.head_dim))
+    a = np.einsum("rhd,hnd->hrn", np.abs(q.astype(np.float64)), np.repeat(kd, g.group, axis=0)).max()
+    a *= (g.softmax_scale or g.head_dim ** -0.5) * 1.4427
+    rel = 2 * 0.6932 * 16 * 2.0 ** -23 * a + 8 * 2.0 ** -22 + (n / 2 + q.shape[0] * g.group) * 2.0 ** -24
+    off = np.abs(np.asarray(got, dtype=np.float64) - want)
+    tol = rel * np.abs(want) + 1e-30
+    assert np.isfinite(got).all() and (off <= tol).all(), f"{what}: {np.nanmax(off / tol):.3f} of the bound ({rel:.2e})"

@@ -1,0 +1,269 @@
+"""Attention that accumulates its weights, through the C ABI, against the definition in 64 bits; and the bounded cache it
+serves: prompt, decode and eviction together.  Tolerances: bounded_ref.assert_attention, assert_scores."""
+import numpy as np
+import pytest
+import torch
+
+from tests import bounded_ref as R
+from tests.gpu_util import dev_q, new_out, to_np
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(name, lens, rows, store, seed, how="add", act=None):
+    """how: "add" (score_in beside score_out), "same" (one buffer), "none" (score_in None)."""
+    n_seq = len(lens)
+    cap = max(lens) + rows + 2
+    cap += -cap % 128
+    slots = n_seq + 2
+    g = R.geom(name, slot_ctx=cap, n_slots=slots)
+    e = R.engine(g)
+    rng = np.random.default_rng(seed)
+    order = rng.permutation(slots)[:n_seq]
+    q, recs = [], []
+    for i, p in enumerate(lens):
+        qq, k, v = R.draw(g, p + rows, rows, seed * 50 + i)
+        q.append(qq)
+        recs.append(R.quantised(g, k, v))
+    # scores of positions that are not held yet, the call's own included, are NaN: they must not be read
+    first = np.full((slots, g.n_kv, cap), np.nan, dtype=np.float32)
+    for i, p in enumerate(lens):
+        first[order[i], :, :p] = 4 * rng.random((g.n_kv, p)) ** 8
+    sin = torch.from_numpy(first).to(e.device)
+    sout = sin if how == "same" else torch.full_like(sin, -3.0)
+    qd, out = dev_q(e, np.stack(q)), new_out(e, n_seq, rows, g.n_head, g.head_dim)
+    pos, part = R.ids(lens, e), e.alloc_track_part(n_seq, rows, sum(lens) + n_seq * rows)
+    a = None if act is None else R.ids(act, e)
+    given = None if how == "none" else sin
+    if store == "paged":
+        pg = R.Paged(e, recs, 0, 128, seed)
+        tab = torch.full((slots, cap // 128), -1, dtype=torch.int32, device=e.device)
+        tab[torch.from_numpy(order.copy()).long(), :pg.table.shape[1]] = pg.table
+        pg.desc.table, pg.desc.n_tables, pg.desc.max_pages = tab.data_ptr(), slots, cap // 128
+        e.attn_track_paged(out, sout, given, qd, pg.desc, pos, part, rows=rows, ktab=R.ids(order, e), act=a)
+    else:
+        kvk, kvv = e.alloc_kv_layer(False, fill=0x7F)
+        for buf, t in ((kvk, 0), (kvv, 1)):
+            R.put(e, buf, {int(s): recs[i] for i, s in enumerate(order)}, False, t)
+        e.attn_track(out, sout, given, qd, kvk, kvv, pos, part, rows=rows, kslot=R.ids(order, e), act=a)
+    torch.cuda.synchronize()
+    assert e.device_status() == 0
+    got, sc = to_np(out), sout.cpu().numpy()
+    rest = np.ones((slots, cap), dtype=bool)
+    for i, p in enumerate(lens):
+        what = f"track {name} {store} rows {rows} at {p}"
+        if act is not None and not act[i]:
+            assert np.isnan(got[i]).all(), what
+            continue
+        rest[order[i], :p + rows] = False
+        R.assert_attention(got[i], R.attend64(g, q[i], *recs[i], p), g, recs[i][1], what)
+        want = R.score64(g, q[i], recs[i][0], p, None if how == "none" else first[order[i]])
+        R.assert_scores(sc[order[i], :, :p + rows], want, g, q[i], recs[i][0], p, what)
+    kept = (first if how == "same" else np.full_like(first, -3.0)).transpose(0, 2, 1)[rest]
+    np.testing.assert_array_equal(sc.transpose(0, 2, 1)[rest], kept)      # everything else is as it was
+
+
+@pytest.mark.parametrize("store", ["slots", "paged"])
+@pytest.mark.parametrize("name", ["B", "B32", "R", "B1", "B8"])
+@pytest.mark.parametrize("how", ["add", "same", "none"])
+def test_one_token_of_many_sequences(name, store, how):
+    _case(name, [0, 1, 62, 63, 64, 127, 500, 2047, 2048, 3001], 1, store, 3, how)
+
+
+@pytest.mark.parametrize("name", ["B", "R"])
+def test_one_token_of_one_sequence(name):
+    for p in (0, 5, 64, 9000, 40001):
+        _case(name, [p], 1, "slots", p + 1, "same")
+
+
+@pytest.mark.parametrize("store", ["slots", "paged"])
+@pytest.mark.parametrize("name,rows", [("B", 2), ("B", 7), ("B", 33), ("B32", 100), ("B", 512), ("R", 3), ("R", 32), ("R", 201),
+                                       ("B8", 50), ("B1", 129)])
+def test_prompt_chunk(name, rows, store):
+    for p, how in ((0, "none"), (1, "add"), (127, "same"), (1700, "same"), (2001, "none")):
+        _case(name, [p], rows, store, rows + p, how)
+
+
+def test_a_long_prompt():
+    _case("B", [16000], 384, "slots", 1, "same")
+    _case("R16", [16000], 40, "paged", 1, "none")
+
+
+def test_idle_sequences_are_left_alone():
+    _case("B", [500, 40, 300, 9], 1, "slots", 5, "same", act=[1, 0, 1, 0])
+    _case("B", [500], 1, "slots", 5, "same", act=[0])
+    for name in ("B", "R"):
+        for rows in (2, 100):
+            _case(name, [600], rows, "paged", 6, "same", act=[0])
+
+
+def test_attention_output_is_the_plain_calls():
+    """What the call adds does not change what it computes: the decode output is battn_decode's, bit for bit."""
+    g = R.geom("B", slot_ctx=4096)
+    e = R.engine(g)
+    for p in (0, 77, 4000):
+        q, k, v = R.draw(g, p + 1, 1, p)
+        recs = R.quantised(g, k, v)
+        kvk, kvv = e.alloc_kv_layer(False, fill=0x7F)
+        R.put(e, kvk, {0: recs}, False, 0)
+        R.put(e, kvv, {0: recs}, False, 1)
+        a, b = new_out(e, 1, 1, g.n_head, g.head_dim), new_out(e, 1, 1, g.n_head, g.head_dim)
+        qd, pos = dev_q(e, q[None]), R.ids([p], e)
+        e.launch_attn_m(a, qd, kvk, kvv, pos, e.alloc_part(1, 1), 1)
+        s = torch.zeros(g.n_kv, 4096, device=e.device)
+        e.attn_track(b, s, s, qd, kvk, kvv, pos, e.alloc_track_part(1, 1, p + 1))
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+
+
+def test_two_graphs_share_a_workspace_and_repeat():
+    """Two captured calls on one workspace, replayed in turn: the same bits every time."""
+    g = R.geom("B", slot_ctx=2048, n_slots=3)
+    e = R.engine(g)
+    lens = [1500, 3, 800]
+    kvk, kvv = (torch.randint(0, 60, (e.kv_layer_bytes(False),), dtype=torch.uint8, device=e.device) for _ in range(2))
+    pos, slots, part = R.ids(lens, e), R.ids([0, 1, 2], e), e.alloc_track_part(3, 100, 4000)
+    q1 = torch.randn(3, 1, g.n_head, g.head_dim, device=e.device).half()
+    q2 = torch.randn(1, 100, g.n_head, g.head_dim, device=e.device).half()
+    o1, o2 = torch.empty_like(q1), torch.empty_like(q2)
+    s1, s2 = (torch.zeros(3, g.n_kv, 2048, device=e.device) for _ in range(2))
+
+    def one():
+        e.attn_track(o1, s1, None, q1, kvk, kvv, pos, part, kslot=slots)
+
+    def two():
+        e.attn_track(o2, s2, None, q2, kvk, kvv, pos[2:], part, rows=100, kslot=slots[2:])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(); two()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    first = [t.clone() for t in (o1, s1, o2, s2)]
+    graphs = []
+    for f in (one, two):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            f()
+        graphs.append(gr)
+    for _ in range(20):
+        for t in (o1, s1, o2, s2):
+            t.fill_(7)
+        graphs[0].replay(); graphs[1].replay()
+        torch.cuda.synchronize()
+        for got, want, clean in ((o1, first[0], None), (o2, first[2], None), (s1, first[1], lens), (s2, first[3], [0, 0, 900])):
+            if clean is None:
+                assert torch.equal(got, want)
+            else:
+                for i, n in enumerate(clean):
+                    assert torch.equal(got[i, :, :n], want[i, :, :n])
+    assert e.device_status() == 0
+
+
+def test_a_workspace_that_is_too_small_for_the_positions():
+    g = R.geom("B", slot_ctx=4096, n_slots=2)
+    e = R.engine(g)
+    kvk, kvv = e.alloc_kv_layer(False, fill=0)
+    q = torch.zeros(2, 1, g.n_head, g.head_dim, dtype=torch.float16, device=e.device)
+    part = e.alloc_track_part(2, 1, 2000)
+    score = torch.full((2, g.n_kv, 4096), 5.0, device=e.device)
+    for lens, status in (([1000, 900], 0), ([4000, 10], 4), ([1, 1], 0)):
+        out = new_out(e, 2, 1, g.n_head, g.head_dim)
+        score.fill_(5.0)
+        e.attn_track(out, score, score, q, kvk, kvv, R.ids(lens, e), part, kslot=R.ids([0, 1], e))
+        torch.cuda.synchronize()
+        assert e.device_status() == status
+        assert bool(torch.isnan(out).all()) == bool(status) and bool((score == 5.0).all()) == bool(status)
+
+
+def test_bad_positions_and_slots_set_the_status_bit():
+    g = R.geom("B", slot_ctx=512, n_slots=2)
+    e = R.engine(g)
+    kvk, kvv = e.alloc_kv_layer(False, fill=0)
+    part = e.alloc_track_part(1, 100, 600)
+    for rows in (1, 4, 100):
+        for p, s in ((-1, 0), (513 - rows, 0), (5, 2), (5, -1)):
+            out = new_out(e, 1, rows, g.n_head, g.head_dim)
+            score = torch.full((2, g.n_kv, 512), 5.0, device=e.device)
+            q = torch.zeros(1, rows, g.n_head, g.head_dim, dtype=torch.float16, device=e.device)
+            e.attn_track(out, score, score, q, kvk, kvv, R.ids([p], e), part, rows=rows, kslot=R.ids([s], e))
+            torch.cuda.synchronize()
+            assert e.device_status() == 1 and torch.isnan(out).all() and (score == 5.0).all(), (rows, p, s)
+
+
+def test_refusals():
+    from bruce_engine_b200 import capi
+    g = R.geom("B", slot_ctx=1024, n_slots=2)
+    e = R.engine(g)
+    cache = e.alloc_kv_layer(False, fill=0)
+    score, part = torch.zeros(2, g.n_kv, 1024, device=e.device), e.alloc_track_part(2, 512, 2048)
+
+    def call(rows=1, n=1, part=part, score=score, into=None, **kw):
+        q = torch.zeros(n, rows, g.n_head, g.head_dim, dtype=torch.float16, device=e.device)
+        e.attn_track(torch.empty_like(q), score if into is None else into, score, q, *cache, R.ids([5] * n, e), part, rows=rows,
+                     kslot=R.ids(range(n), e))
+
+    call()
+    for code, kw in ((capi.ERR_CAPACITY, dict(rows=2, n=2)), (capi.ERR_CAPACITY, dict(rows=513)),
+                     (capi.ERR_CAPACITY, dict(part=part[:256])), (capi.ERR_CAPACITY, dict(rows=100, part=part[:4096])),
+                     (capi.ERR_ARG, dict(part=part[8:])),
+                     (capi.ERR_ARG, dict(into=torch.zeros(score.numel() + 1, device=e.device)[1:]))):
+        with pytest.raises(capi.BattnError) as err:
+            call(**kw)
+        assert err.value.code == code, kw
+    for kw in (dict(score=score[:1]), dict(score=score.double()), dict(score=score.transpose(1, 2))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    import ctypes
+    n = ctypes.c_size_t()
+    for args in ((0, 1, 1), (1, 0, 1), (1, 1, -1)):
+        assert e.lib.battn_track_workspace_bytes(e.h, *args, n) == capi.ERR_ARG
+    torch.cuda.synchronize()
+    assert e.device_status() == 0
+
+
+@pytest.mark.parametrize("name", ["B", "R"])
+def test_a_conversation_in_a_bounded_cache(name):
+    """A prompt of 300 tokens, cut to 128, then 120 tokens with a trim whenever 160 are held: append, attend and accumulate,
+    evict.  Every step is checked against 64 bits, starting from the scores the previous step left."""
+    budget, n_sink, n_recent, limit = 128, 4, 32, 160
+    g = R.geom(name, slot_ctx=512, n_slots=2)
+    e = R.engine(g)
+    q, k, v = R.draw(g, 420, 420, 77)
+    kvk, kvv = e.alloc_kv_layer(False, fill=0x7F)
+    slot, pos = R.ids([1], e), R.ids([0], e)
+    score = torch.full((2, g.n_kv, 512), float("nan"), device=e.device)
+    kept = torch.zeros(1, g.n_kv, budget, dtype=torch.int32, device=e.device)
+    part, epart = e.alloc_track_part(1, 300, 512), e.alloc_evict_part(1)
+    krec, vrec = (np.zeros((g.n_kv, 0, g.rec), dtype=np.uint8) for _ in range(2))
+    held, at = 0, 0
+    while at < 420:
+        rows = 300 if at == 0 else 1
+        before = score.cpu().numpy()[1]
+        kd, vd = (torch.from_numpy(x[at:at + rows]).to(e.device) for x in (k, v))
+        qd = torch.from_numpy(q[at:at + rows]).to(e.device).to(e.q_torch)[None].contiguous()
+        out = new_out(e, 1, rows, g.n_head, g.head_dim)
+        e.qkv_prep_store(kd, vd, kvk, kvv, pos, kslot=slot, rows=rows)
+        e.attn_track(out, score, score, qd, kvk, kvv, pos, part, rows=rows, kslot=slot)
+        new = R.quantised(g, k[at:at + rows], v[at:at + rows])
+        krec, vrec = np.concatenate([krec, new[0]], 1), np.concatenate([vrec, new[1]], 1)
+        torch.cuda.synchronize()
+        what = f"token {at}"
+        R.assert_attention(to_np(out)[0], R.attend64(g, q[at:at + rows], krec, vrec, held), g, vrec, what)
+        now = score.cpu().numpy()[1]
+        R.assert_scores(now[:, :held + rows], R.score64(g, q[at:at + rows], krec, held, before), g, q[at:at + rows], krec, held, what)
+        pos += rows
+        held, at = held + rows, at + rows
+        if held >= limit:
+            e.evict(kvk, kvv, score, kept, pos, pos, epart, budget, n_sink=n_sink, n_recent=n_recent, kslot=slot)
+            torch.cuda.synchronize()
+            idx = np.stack([R.evict_list(now[h, :held], budget, n_sink, n_recent) for h in range(g.n_kv)])
+            np.testing.assert_array_equal(kept.cpu().numpy()[0], idx)
+            h = np.arange(g.n_kv)[:, None]
+            krec, vrec, held = krec[h, idx], vrec[h, idx], budget
+            assert int(pos[0]) == budget
+            np.testing.assert_array_equal(score.cpu().numpy()[1, :, :budget], now[h, idx])
+            got = kvk.cpu().numpy().reshape(2, g.n_kv, 512, g.rec)[1, :, :budget]
+            assert (got == krec).all()
+    assert e.device_status() == 0
