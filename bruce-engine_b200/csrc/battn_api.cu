@@ -104,10 +104,6 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     }
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_TRACK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(tr::k_track_chunk<HD>, tr::ChunkCfg<HD>::SMEM)) != cudaSuccess) return e;
-    h->track_ctas_per_sm = 1;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&h->track_ctas_per_sm, (const void*)tr::k_track_chunk<HD>, tr::CTHREADS,
-                                                      tr::ChunkCfg<HD>::SMEM);
-    if (e != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_select, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::SMEM)) != cudaSuccess) return e;
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
@@ -150,14 +146,15 @@ inline int exact_default_splits(int rows) { return rows > 64 ? 2 : (rows > 8 ? 8
 // for few kv heads (64 CTAs for a 512-row chunk in the 16/4/256 geometry); each (M tile, kv head) is then shared by several CTAs that take
 // contiguous shares of the key tiles and leave split records for the merge kernel.  Positions are device-resident,
 // so the choice depends on the chunk shape only.
-inline int prefill_splits(const battn_handle* h, int rows, int is_swa) {
+inline int prefill_splits(const battn_handle* h, int rows, int is_swa, int var = VAR_PLAIN) {
     const Geom& g = h->g;
     const int ctas = ((rows + 128 / g.G - 1) / (128 / g.G)) * g.Hkv;
     int s = h->num_sms / ctas;
     // a share should keep at least 16 key tiles of 64, or the merge costs more than the split saves; a
     // sliding-window layer never has more than window/64 + 1 tiles per M tile
-    if (is_swa && s > g.W / (64 * 16)) s = g.W / (64 * 16);
-    return s < 1 ? 1 : (s > 8 ? 8 : s);
+    const int share = var == VAR_SINK ? 6 : 16, most = var == VAR_TRACK ? 32 : 8;
+    if (is_swa && s > g.W / (64 * share)) s = g.W / (64 * share);
+    return s < 1 ? 1 : (s > most ? most : s);
 }
 
 inline size_t exact_workspace(const battn_handle* h, int n_seq, int rows, int nsplit) {
@@ -286,7 +283,7 @@ struct StepVariant {
     SinkView sink;               // VAR_SINK
     float* scores;               // VAR_TRACK, see fd::Params
     int sc_tiles;
-    int cph;                     // out, VAR_TRACK: the work cut the call took
+    tr::StepParams* track;       // VAR_TRACK: what the accumulation needs besides
 };
 
 template <int HD, int NT>
@@ -381,14 +378,25 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
     M.n_rows = n_seq * rows; M.rows = rows; M.Hq = g.Hq; M.Hkv = g.Hkv; M.G = g.G;
     M.count = 0; M.log2_domain = 1; M.out_f16 = g.out_f16; M.hdr = P.hdr; M.status = h->d_status;
     M.cph = P.cph;
-    if (sv) sv->cph = P.cph;
     if (P.early && fd_grid > 0 && n_seq == 1 && var == VAR_PLAIN) {
         // the merge recomputes the cut from the positions while it waits for the decode kernel
         M.pre_grid = fd_grid; M.pre_tile = fd::TILE;
         M.pos = pos; M.kslot = kslot; M.act = act; M.is_swa = is_swa; M.W = g.W; M.slot_ctx = P.slot_ctx; M.n_slots = P.n_slots;
     }
     if (xv) M.xchg = *xv;
-    if (g.HD == 128) e = launch_pdl(k_merge_balanced<128>, dim3(n_seq * rows * g.Hq), dim3(MERGE_B_THREADS), 0, st, M);
+    // the variants' merge: a warp per (row, head) once the blocks of the other form are more than one wave
+    const int items = n_seq * rows * g.Hq, per_block = MERGE_M_THREADS / 32;
+    const bool many = var != VAR_PLAIN && items > h->num_sms * 2;
+    if (var == VAR_TRACK) {
+        tr::StepMerge T{M, *sv->track, many ? (items + per_block - 1) / per_block : items};
+        T.step.hdr = P.hdr; T.step.part = P.part; T.step.scores = P.scores; T.step.cph = P.cph;
+        const size_t cum = (size_t)(n_seq + 1) * sizeof(int);
+        const dim3 grid(T.merge_blocks + h->num_sms * (many ? 8 : 2));
+        if (many) e = launch_pdl(g.HD == 128 ? tr::k_merge_track_many<128> : tr::k_merge_track_many<256>, grid, dim3(MERGE_M_THREADS), cum, st, T);
+        else      e = launch_pdl(g.HD == 128 ? tr::k_merge_track_few<128> : tr::k_merge_track_few<256>, grid, dim3(MERGE_B_THREADS), cum, st, T);
+    }
+    else if (many) e = launch_pdl(g.HD == 128 ? k_merge_many<128> : k_merge_many<256>, dim3((items + per_block - 1) / per_block), dim3(MERGE_M_THREADS), 0, st, M);
+    else if (g.HD == 128) e = launch_pdl(k_merge_balanced<128>, dim3(n_seq * rows * g.Hq), dim3(MERGE_B_THREADS), 0, st, M);
     else             e = launch_pdl(k_merge_balanced<256>, dim3(n_seq * rows * g.Hq), dim3(MERGE_B_THREADS), 0, st, M);
     h->launches += 2;
     if (e == cudaSuccess) e = cudaGetLastError();
@@ -430,7 +438,7 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
                (h->kvw_kind == 3 && h->kvw_cache != (const void*)kvk));
     h->kvw_kind = 0;
     const int MR = 128 / g.G;
-    P.nsplit = prefill_splits(h, rows, is_swa || var == VAR_SINK);
+    P.nsplit = prefill_splits(h, rows, is_swa || var == VAR_SINK, var);
     P.recs = (P.nsplit > 1 || gn) ? reinterpret_cast<float*>(ws) : nullptr;
     const dim3 grid((rows + MR - 1) / MR, g.Hkv, P.nsplit);
     {
@@ -1005,7 +1013,7 @@ static int attend_sinks_impl(battn_handle* h, void* out, const void* q, const ui
     const DeviceScope dev(h->device);
     cudaStream_t st = (cudaStream_t)stream;
     if (rows <= MAX_VERIFY && rows * g.G <= 32) {
-        StepVariant sv{VAR_SINK, cv.sink, nullptr, 0, 0};
+        StepVariant sv{VAR_SINK, cv.sink, nullptr, 0, nullptr};
         return launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, rows, is_swa, st, nullptr, nullptr, 0, pv,
                             nullptr, nullptr, nullptr, &sv);
     }
@@ -1037,8 +1045,9 @@ struct TrackChunkWs {
 static TrackChunkWs track_chunk_workspace(const battn_handle* h, int rows) {
     const size_t per = (size_t)rows * h->g.Hq;
     TrackChunkWs w;
-    w.stats = align_up(prefill_workspace(h, rows), 256);
-    w.lse = w.stats + align_up(per * prefill_splits(h, rows, 0) * sizeof(float2), 256);
+    const int splits = prefill_splits(h, rows, 0, VAR_TRACK);
+    w.stats = align_up(exact_workspace(h, 1, rows, splits), 256);
+    w.lse = w.stats + align_up(per * splits * sizeof(float2), 256);
     w.total = w.lse + align_up(per * sizeof(float), 256);
     return w;
 }
@@ -1069,17 +1078,13 @@ static int attend_track_impl(battn_handle* h, void* out, float* score_out, const
         const size_t base = align_up(fd_workspace(h, n_seq, 1).total, 256), tile = (size_t)fd::TILE * g.G * sizeof(float);
         if (ws_bytes < base + tile) return BATTN_ERR_CAPACITY;
         const size_t tiles = (ws_bytes - base) / tile;
-        StepVariant sv{VAR_TRACK, {}, reinterpret_cast<float*>(w + base), (int)std::min<size_t>(tiles, 0x7fffffff), 0};
-        rc = launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, 1, 0, st, nullptr, nullptr, 0, pv, nullptr,
-                          nullptr, nullptr, &sv);
-        if (rc) return rc;
-        const FdWs fw = fd_workspace(h, n_seq, 1);
-        tr::StepParams P;
-        P.hdr = reinterpret_cast<const int*>(ws); P.part = reinterpret_cast<const float*>(w + fw.hdr_bytes);
-        P.scores = sv.scores; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot;
-        P.n_seq = n_seq; P.Hkv = g.Hkv; P.G = g.G; P.HD = g.HD; P.cph = sv.cph;
+        tr::StepParams P{};
+        P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot;
+        P.n_seq = n_seq; P.Hkv = g.Hkv; P.G = g.G; P.HD = g.HD;
         P.stride = pv ? (size_t)pv->capacity : (size_t)g.slot_ctx;
-        e = launch_pdl(tr::k_track_step, dim3(h->num_sms * 2), dim3(tr::STEP_THREADS), (n_seq + 1) * sizeof(int), st, P);
+        StepVariant sv{VAR_TRACK, {}, reinterpret_cast<float*>(w + base), (int)std::min<size_t>(tiles, 0x7fffffff), &P};
+        return launch_flash(h, out, nullptr, q, kvk, kvv, pos, kslot, act, ws, n_seq, 1, 0, st, nullptr, nullptr, 0, pv, nullptr,
+                            nullptr, nullptr, &sv);
     } else {
         if (n_seq != 1) return BATTN_ERR_CAPACITY;
         const TrackChunkWs cw = track_chunk_workspace(h, rows);
@@ -1093,7 +1098,7 @@ static int attend_track_impl(battn_handle* h, void* out, float* score_out, const
         P.pstride = pv ? pv->capacity : g.slot_ctx; P.n_slots = pv ? pv->n_tables : g.n_slots;
         P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
         if (pv) P.pg = pv->pg;
-        const dim3 grid(h->num_sms * std::max(1, h->track_ctas_per_sm)), block(tr::CTHREADS);
+        const dim3 grid(h->num_sms), block(tr::CTHREADS);
         e = g.HD == 128 ? launch_pdl(tr::k_track_chunk<128>, grid, block, tr::ChunkCfg<128>::SMEM, st, P)
                         : launch_pdl(tr::k_track_chunk<256>, grid, block, tr::ChunkCfg<256>::SMEM, st, P);
     }
@@ -1126,13 +1131,6 @@ int battn_evict_workspace_bytes(const battn_handle* h, int n_seq, size_t* out_by
     return BATTN_OK;
 }
 
-// CTAs per cluster for `items` clusters: as many as the SMs have room for, a power of two up to the portable limit
-static int evict_cluster(const battn_handle* h, int items) {
-    int c = 1;
-    while (c < ev::MAX_CLUSTER && items * c * 2 <= h->num_sms) c *= 2;
-    return c;
-}
-
 static int evict_impl(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score, int* kept, int* pos_out, const int* pos,
                       const int* kslot, const int* kslot_dst, const int* act, void* ws, int budget, int n_sink, int n_recent,
                       int n_seq, void* stream, const PagedView* pv) {
@@ -1158,13 +1156,19 @@ static int evict_impl(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score,
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2; cfg.stream = st;
-    int c = evict_cluster(h, n_seq * g.Hkv);
-    attr[0].val.clusterDim.x = c;
-    cfg.gridDim = dim3(n_seq * c, g.Hkv); cfg.blockDim = dim3(ev::SEL_THREADS); cfg.dynamicSmemBytes = ev::KEYS_SMEM * 4;
+    // selection: a cluster per (sequence, kv head), a power of two up to the portable limit -- CTAs for the longest
+    // sequence the cache can hold, as long as the SMs have room; a cluster uses as many of them as its sequence needs
+    int c = 1;
+    while (c < ev::MAX_CLUSTER && n_seq * g.Hkv * c * 2 <= h->num_sms && c * ev::KEYS_PER_CTA < P.pstride) c *= 2;
+    P.cluster = attr[0].val.clusterDim.x = c;
+    P.keys = std::min(ev::KEYS_SMEM, (std::max(ev::KEYS_PER_CTA, (P.pstride + c - 1) / c) + 3) & ~3);
+    cfg.gridDim = dim3(n_seq * c, g.Hkv); cfg.blockDim = dim3(ev::SEL_THREADS); cfg.dynamicSmemBytes = (size_t)P.keys * 4;
     cudaError_t e = cudaLaunchKernelEx(&cfg, ev::k_evict_select, P);
     if (e != cudaSuccess) return cuda_fail(h, e);
-    c = evict_cluster(h, n_seq * g.Hkv * 2);
-    attr[0].val.clusterDim.x = c;
+    // move: as many CTAs as a budget has rounds, so that a batch spreads evenly too
+    const int round = g.HD == 128 ? ev::MoveCfg<128>::ROUND : ev::MoveCfg<256>::ROUND;
+    for (c = 1; c < ev::MAX_CLUSTER && c * round < budget; ) c *= 2;
+    P.cluster = attr[0].val.clusterDim.x = c;
     cfg.gridDim = dim3(n_seq * c, g.Hkv, 2); cfg.blockDim = dim3(ev::MOVE_THREADS);
     cfg.dynamicSmemBytes = g.HD == 128 ? ev::MoveCfg<128>::SMEM : ev::MoveCfg<256>::SMEM;
     e = g.HD == 128 ? cudaLaunchKernelEx(&cfg, ev::k_evict_move<128>, P) : cudaLaunchKernelEx(&cfg, ev::k_evict_move<256>, P);

@@ -9,8 +9,6 @@
 // target positions of the whole cluster, loads all of its sources into shared memory, and stores after a cluster barrier.
 // What it overwrites lies below the targets of the next round, and the sources of every later round lie at or above them.
 #pragma once
-#include <cooperative_groups.h>
-
 #include "common.cuh"
 
 namespace battn {
@@ -18,8 +16,10 @@ namespace ev {
 
 constexpr int MAX_CLUSTER = 8;              // the portable limit
 constexpr int SEL_THREADS = 1024, MOVE_THREADS = 256;
-constexpr int KEYS_SMEM = 40 * 1024;        // keys a CTA keeps in shared memory (160 KB); a longer share re-reads the rest
-constexpr int BINS = 2048;
+constexpr int KEYS_SMEM = 40 * 1024;        // keys a CTA keeps in shared memory at most (160 KB); a longer share re-reads the rest
+// Candidates that are worth another CTA of the cluster: up to here a pass over them is shorter than the cluster barriers
+// (4160 positions, one CTA of eight: 23 -> 12 us)
+constexpr int KEYS_PER_CTA = 8192;
 
 struct Params {
     uint8_t* kvk;
@@ -34,9 +34,23 @@ struct Params {
     const int* act;
     int n_seq, budget, n_sink, n_recent;
     int Hkv, pstride, n_slots;
+    int cluster;         // CTAs per cluster of this launch
+    int keys;            // k_evict_select: keys its shared memory holds
     int* status;
     Paging pg;
 };
+
+// Cluster barriers (CTAs that have left count as arrived) and reads of another CTA's shared memory.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() { cluster_arrive(); cluster_wait(); }
+template <int N>
+__device__ __forceinline__ void load_rank(const uint32_t* p, int r, uint32_t (&v)[N]) {
+    uint32_t ra;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(p)), "r"(r));
+    if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(ra) : "memory");
+    else                  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[0]) : "r"(ra) : "memory");
+}
 
 // Scores as integers of the same order: NaN below everything, the two zeros alike.
 __device__ __forceinline__ uint32_t ordered(float f) {
@@ -68,16 +82,61 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp, uin
     return x - v + (warp ? before : 0u);
 }
 
+// One pass of the descent over BITS bits at SHIFT.  `hist` holds this CTA's counts of the keys that match the prefix so
+// far; every CTA adds up the cluster's counts itself and finds the same bin.  Counts of the CTAs before this one are kept
+// too: above the bin they end up in `gt_low`, in the last pass the bin's own are `eq_low`.
+template <int SHIFT, int BITS>
+__device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_t* s_warp, volatile uint32_t* s_found,
+                                        uint32_t& prefix, uint32_t& need, uint32_t& gt_low, uint32_t& eq_low) {
+    constexpr int PER = (1 << BITS) / SEL_THREADS;               // bins per thread, from the highest down
+    const int top = (1 << BITS) - PER * ((int)threadIdx.x + 1);  // lowest of this thread's bins
+    uint32_t c[PER], low[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) c[e] = low[e] = 0;
+    if (C > 1) {
+        cluster_sync();
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) {
+            if (r >= C) break;
+            uint32_t v[PER];
+            load_rank<PER>(hist + top, r, v);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) { c[e] += v[e]; low[e] += r < rank ? v[e] : 0u; }
+        }
+    } else {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < PER; ++e) c[e] = hist[top + e];
+    }
+    uint32_t sum = 0, tot;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum += c[e];
+    uint32_t before = block_scan(sum, s_warp, tot);
+#pragma unroll
+    for (int e = PER - 1; e >= 0; --e) {
+        if (before < need && before + c[e] >= need) { s_found[0] = top + e; s_found[1] = before; }
+        before += c[e];
+    }
+    __syncthreads();
+    const uint32_t bin = s_found[0];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        if (top + e > (int)bin) gt_low += low[e];
+        if (SHIFT == 0 && top + e == (int)bin) eq_low += low[e];
+    }
+    prefix = (prefix << BITS) | bin;
+    need -= s_found[1];
+}
+
 __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P) {
-    namespace cg = cooperative_groups;
-    extern __shared__ uint32_t s_key[];              // KEYS_SMEM keys of this CTA's share
-    __shared__ uint32_t s_hist[BINS], s_warp[32];
-    __shared__ uint32_t s_bin, s_above, s_gt, s_eq;
+    extern __shared__ uint32_t s_key[];              // P.keys keys of this CTA's share
+    __shared__ __align__(8) uint32_t s_hist[2048 + 2048 + 1024];
+    __shared__ uint32_t s_warp[32], s_found[3][2], s_low[2];
     __shared__ int s_clash;
-    const cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    const int i = blockIdx.x / C, kvh = blockIdx.y, tid = threadIdx.x;
-    if (tid == 0) s_clash = 0;
+    const int CL = P.cluster, rank = (int)blockIdx.x % CL;
+    const int i = blockIdx.x / CL, kvh = blockIdx.y, tid = threadIdx.x;
+    for (int b = tid; b < 2048 + 2048 + 1024; b += SEL_THREADS) s_hist[b] = 0;
+    if (tid == 0) { s_clash = 0; s_low[0] = s_low[1] = 0; }
     pdl_wait();
     pdl_trigger();
     __syncthreads();
@@ -91,7 +150,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
         const int sj = P.kslot ? P.kslot[j] : 0, dj = P.kslot_dst ? P.kslot_dst[j] : sj;
         if (dj == dst || sj == dst) s_clash = 1;
     }
-    __syncthreads();
+    if (P.n_seq > 1) __syncthreads();
     bad = bad || s_clash;
     const int stay = min(n, P.budget);
     if (kvh == 0 && rank == 0 && tid == 0) {
@@ -101,7 +160,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
     if (idle || bad) return;                         // the whole cluster
 
     int* kept = P.kept + ((size_t)i * P.Hkv + kvh) * P.budget;
-    const int gtid = rank * SEL_THREADS + tid, gthreads = C * SEL_THREADS;
+    const int gtid = rank * SEL_THREADS + tid, gthreads = CL * SEL_THREADS;
     if (n <= P.budget) {
         for (int j = gtid; j < P.budget; j += gthreads) kept[j] = j < n ? j : -1;
         return;
@@ -110,105 +169,98 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
     for (int j = gtid; j < P.n_recent; j += gthreads) kept[P.budget - P.n_recent + j] = n - P.n_recent + j;
     const int cand = n - P.n_sink - P.n_recent, m = P.budget - P.n_sink - P.n_recent;
     if (m == 0) return;
-    // ---- this CTA's share of the candidates, as keys ---------------------------------------------------------------
-    const float* score = P.score + ((size_t)src * P.Hkv + kvh) * P.pstride + P.n_sink;
+    // ---- this CTA's share of the candidates, as keys; CTAs that are not needed leave (barriers count who is left) -----
+    const int C = min(CL, (cand + KEYS_PER_CTA - 1) / KEYS_PER_CTA);
+    if (rank >= C) return;
     const int per = ((cand + C - 1) / C + 3) & ~3;
     const int a = min(rank * per, cand), len = min(per, cand - a);
-    score += a;
-    for (int j = tid; j < min(len, KEYS_SMEM); j += SEL_THREADS) s_key[j] = ordered(score[j]);
-    auto key = [&](int j) { return j < KEYS_SMEM ? s_key[j] : ordered(score[j]); };
-
-    // ---- the m-th best key, 11 + 11 + 10 bits --------------------------------------------------------------------------
-    uint32_t prefix = 0, need = (uint32_t)m;
+    const float* score = P.score + ((size_t)src * P.Hkv + kvh) * P.pstride + P.n_sink + a;
+    const int held = min(len, P.keys);
+    auto key = [&](int j) { return j < held ? s_key[j] : ordered(__ldg(score + j)); };
+    constexpr int UN = 8;
+    for (int j0 = tid; j0 < len; j0 += UN * SEL_THREADS) {       // the scores' one trip, and the first pass's counts
+        float v[UN];
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-        for (int b = tid; b < bins; b += SEL_THREADS) s_hist[b] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += SEL_THREADS) {
-            const uint32_t k = key(j);
-            if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
-        }
-        cl.sync();
-        // from the highest bin down: thread t adds up bins - 1 - per_t * t ...
-        const int per_t = bins / SEL_THREADS;
-        uint32_t c[2] = {0, 0};
-        for (int r = 0; r < C; ++r) {
-            const uint32_t* h = cl.map_shared_rank(s_hist, r);
+        for (int u = 0; u < UN; ++u) v[u] = j0 + u * SEL_THREADS < len ? __ldg(score + j0 + u * SEL_THREADS) : 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (e < per_t) c[e] += h[bins - 1 - per_t * tid - e];
+        for (int u = 0; u < UN; ++u) {
+            const int j = j0 + u * SEL_THREADS;
+            if (j < len) {
+                const uint32_t k = ordered(v[u]);
+                if (j < held) s_key[j] = k;
+                atomicAdd(&s_hist[k >> 21], 1u);
+            }
         }
-        uint32_t tot, before = block_scan(c[0] + c[1], s_warp, tot);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (e < per_t && before < need && before + c[e] >= need) { s_bin = bins - 1 - per_t * tid - e; s_above = before; }
-            before += c[e];
-        }
-        cl.sync();                                   // every CTA has read this one's counts
-        prefix = (prefix << bits) | s_bin;
-        need -= s_above;
     }
-    // ---- better than the m-th, or equal and among the first `need` equal ones: the list, in order -----------------------
-    const uint32_t T = prefix;
-    if (tid == 0) { s_gt = 0; s_eq = 0; }
-    __syncthreads();
-    uint32_t gt = 0, eq = 0;
+    // ---- the m-th best key ------------------------------------------------------------------------------------------------
+    uint32_t T = 0, need = (uint32_t)m, gt_low = 0, eq_low = 0;
+    descend<21, 11>(s_hist, C, rank, s_warp, s_found[0], T, need, gt_low, eq_low);
     for (int j = tid; j < len; j += SEL_THREADS) {
         const uint32_t k = key(j);
-        gt += k > T; eq += k == T;
+        if ((k >> 21) == T) atomicAdd(&s_hist[2048 + ((k >> 10) & 2047)], 1u);
     }
-    gt = __reduce_add_sync(0xffffffffu, gt);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    if ((tid & 31) == 0) { atomicAdd(&s_gt, gt); atomicAdd(&s_eq, eq); }
-    cl.sync();
+    descend<10, 11>(s_hist + 2048, C, rank, s_warp, s_found[1], T, need, gt_low, eq_low);
+    for (int j = tid; j < len; j += SEL_THREADS) {
+        const uint32_t k = key(j);
+        if ((k >> 10) == T) atomicAdd(&s_hist[4096 + (k & 1023)], 1u);
+    }
+    descend<0, 10>(s_hist + 4096, C, rank, s_warp, s_found[2], T, need, gt_low, eq_low);
+    if (C > 1) cluster_arrive();                                 // this CTA reads no other's counts any more
+    // ---- better than the m-th, or equal and among the first `need` equal ones: the list, in order -----------------------
     uint32_t gt0 = 0, eq0 = 0;
-    for (int r = 0; r < rank; ++r) { gt0 += *cl.map_shared_rank(&s_gt, r); eq0 += *cl.map_shared_rank(&s_eq, r); }
+    if (C > 1) {
+        gt_low = __reduce_add_sync(0xffffffffu, gt_low);
+        eq_low = __reduce_add_sync(0xffffffffu, eq_low);
+        if ((tid & 31) == 0) { atomicAdd(&s_low[0], gt_low); atomicAdd(&s_low[1], eq_low); }
+        __syncthreads();
+        gt0 = s_low[0]; eq0 = s_low[1];
+    }
     kept += P.n_sink;
     for (int base = 0; base < len; base += 4 * SEL_THREADS) {
+        const int j0 = base + 4 * tid;
         uint32_t k[4], mine = 0;                     // two counts of 16 bits: better, equal
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int j = base + 4 * tid + e;
-            k[e] = j < len ? key(j) : 0u;
-            if (j < len) mine += (k[e] > T ? 0x10000u : 0u) + (k[e] == T ? 1u : 0u);
+            k[e] = j0 + e < len ? key(j0 + e) : 0u;
+            if (j0 + e < len) mine += (k[e] > T ? 0x10000u : 0u) + (k[e] == T ? 1u : 0u);
         }
         uint32_t tot;
         const uint32_t at = block_scan(mine, s_warp, tot);
         uint32_t g = gt0 + (at >> 16), q = eq0 + (at & 0xFFFFu);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int j = base + 4 * tid + e;
-            if (j >= len) break;
-            if (k[e] > T) { kept[g + min(q, need)] = P.n_sink + a + j; ++g; }
-            else if (k[e] == T) { if (q < need) kept[g + q] = P.n_sink + a + j; ++q; }
+            if (j0 + e >= len) break;
+            if (k[e] > T) { kept[g + min(q, need)] = P.n_sink + a + j0 + e; ++g; }
+            else if (k[e] == T) { if (q < need) kept[g + q] = P.n_sink + a + j0 + e; ++q; }
         }
         gt0 += tot >> 16; eq0 += tot & 0xFFFFu;
     }
-    cl.sync();                                       // this CTA's counts are read by the others
+    if (C > 1) cluster_wait();                       // the others have read this CTA's counts
 }
 
 template <int HD>
 struct MoveCfg {
     static constexpr int REC = HD + HD / 16, WORDS = REC / 8;
-    static constexpr int ROUND = HD == 128 ? 512 : 256;          // records of a CTA in a round
-    static constexpr int SMEM = ROUND * (REC + 8 + 4);           // records, source offsets, scores
+    static constexpr int ROUND = HD == 128 ? 256 : 128;          // records of a CTA in a round (34 KB), two rounds in flight
+    static constexpr int BUF = ROUND * (REC + 4);                // records and scores
+    static constexpr int SMEM = 2 * BUF;
+    static_assert(ROUND * REC % 16 == 0 && BUF % 16 == 0, "16-byte stores");
 };
 
 __device__ __forceinline__ void copy8_async(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copy4_async(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 
+// Sources are 8-byte aligned only (a record is 136 or 272 bytes), targets are one run of 16-byte pieces per round and page.
 template <int HD>
 __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     using C = MoveCfg<HD>;
-    namespace cg = cooperative_groups;
     extern __shared__ __align__(16) uint8_t smem[];
-    uint2* s_rec = reinterpret_cast<uint2*>(smem);
-    long long* s_off = reinterpret_cast<long long*>(smem + C::ROUND * C::REC);      // byte offset of the source, -1: stays
-    float* s_score = reinterpret_cast<float*>(s_off + C::ROUND);
-    const cg::cluster_group cl = cg::this_cluster();
-    const int nb = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    __shared__ long long s_off[2][C::ROUND];         // byte offset of the source record
+    const int nb = P.cluster, rank = (int)blockIdx.x % nb;
     const int i = blockIdx.x / nb, kvh = blockIdx.y, tid = threadIdx.x;
     const bool isv = blockIdx.z != 0;
     pdl_wait();
@@ -219,33 +271,58 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     const int src = P.kslot ? P.kslot[i] : 0, dst = P.kslot_dst ? P.kslot_dst[i] : src;
     const int* kept = P.kept + ((size_t)i * P.Hkv + kvh) * P.budget;
     uint8_t* cache = isv ? P.kvv : P.kvk;
-    float* sc_src = P.score + ((size_t)src * P.Hkv + kvh) * P.pstride;
+    const float* sc_src = P.score + ((size_t)src * P.Hkv + kvh) * P.pstride;
     float* sc_dst = P.score + ((size_t)dst * P.Hkv + kvh) * P.pstride;
-    for (int j0 = 0; j0 < stay; j0 += nb * C::ROUND) {
-        const int first = j0 + rank * C::ROUND, cnt = max(0, min(C::ROUND, stay - first));
+    const int rounds = (stay + nb * C::ROUND - 1) / (nb * C::ROUND);
+    // loads of a round into its buffer; false where every record of this CTA's part is where it belongs already
+    auto load = [&](int rd) {
+        const int first = (rd * nb + rank) * C::ROUND, cnt = max(0, min(C::ROUND, stay - first));
+        uint8_t* buf = smem + (rd & 1) * C::BUF;
+        bool moves = false;
         for (int r = tid; r < cnt; r += MOVE_THREADS) {
             const int from = kept[first + r];
-            const bool same = from == first + r && src == dst;
-            s_off[r] = same ? -1 : (long long)(kv_rec_index(P.pg, src, kvh, P.Hkv, P.pstride, from, P.status) * (size_t)C::REC);
-            if (!isv && !same) s_score[r] = sc_src[from];
+            moves |= from != first + r || src != dst;
+            s_off[rd & 1][r] = (long long)(kv_rec_index(P.pg, src, kvh, P.Hkv, P.pstride, from, P.status) * (size_t)C::REC);
+            if (!isv) copy4_async(buf + C::ROUND * C::REC + 4 * r, sc_src + from);
         }
-        __syncthreads();
-        for (int w = tid; w < cnt * C::WORDS; w += MOVE_THREADS) {
-            const int r = w / C::WORDS, c = w - r * C::WORDS;
-            if (s_off[r] >= 0) copy8_async(&s_rec[w], cache + s_off[r] + 8 * c);
+        moves = __syncthreads_or(moves);
+        if (moves)
+            for (int w = tid; w < cnt * C::WORDS; w += MOVE_THREADS) {
+                const int r = w / C::WORDS, c = w - r * C::WORDS;
+                copy8_async(buf + 8 * w, cache + s_off[rd & 1][r] + 8 * c);
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return moves;
+    };
+    bool moves = load(0);
+    for (int rd = 0; rd < rounds; ++rd) {
+        bool next = false;
+        if (rd + 1 < rounds) next = load(rd + 1);    // what is stored below lies under every source of this round
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (nb > 1) cluster_sync(); else __syncthreads();        // every source of round rd has been read
+        if (moves) {
+            const int first = (rd * nb + rank) * C::ROUND, cnt = min(C::ROUND, stay - first);
+            const uint8_t* buf = smem + (rd & 1) * C::BUF;
+            for (int w = tid; w < cnt * C::REC / 16; w += MOVE_THREADS) {
+                // (an odd last record leaves a half piece, stored below; a piece never spans two pages)
+                const int r = 16 * w / C::REC;
+                uint8_t* to = cache + kv_rec_index(P.pg, dst, kvh, P.Hkv, P.pstride, first + r, P.status) * (size_t)C::REC +
+                              (16 * w - r * C::REC);
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(buf + 16 * w);
+            }
+            if (tid == 0 && (cnt * C::REC & 8)) {
+                const int at = cnt * C::REC - 8;
+                uint8_t* to = cache + kv_rec_index(P.pg, dst, kvh, P.Hkv, P.pstride, first + cnt - 1, P.status) * (size_t)C::REC +
+                              (C::REC - 8);
+                *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(buf + at);
+            }
+            if (!isv)
+                for (int r = tid; r < cnt; r += MOVE_THREADS)
+                    sc_dst[first + r] = reinterpret_cast<const float*>(buf + C::ROUND * C::REC)[r];
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        cl.sync();                                   // every source of this round has been read
-        for (int w = tid; w < cnt * C::WORDS; w += MOVE_THREADS) {
-            const int r = w / C::WORDS, c = w - r * C::WORDS;
-            if (s_off[r] < 0) continue;
-            const size_t to = kv_rec_index(P.pg, dst, kvh, P.Hkv, P.pstride, first + r, P.status) * (size_t)C::REC;
-            *reinterpret_cast<uint2*>(cache + to + 8 * c) = s_rec[w];
-        }
-        if (!isv)
-            for (int r = tid; r < cnt; r += MOVE_THREADS)
-                if (s_off[r] >= 0) sc_dst[first + r] = s_score[r];
-        __syncthreads();                             // the buffers are free again
+        moves = next;
+        __syncthreads();                             // the buffer is free again
     }
 }
 

@@ -262,13 +262,13 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_merge(const MergeParams P) {
 
     if (P.stats && warp == 0) {
         const size_t si = (size_t)rowidx * P.Hq + hq, step = (size_t)P.n_rows * P.Hq;
-        float2 st = lane < count ? P.stats[si + lane * step] : make_float2(NEG_BIG, 0.f);       // at most 8 splits
+        float2 st = lane < count ? P.stats[si + lane * step] : make_float2(NEG_BIG, 0.f);       // at most 32 splits
         float M = st.x;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         float L = st.y * fast_exp2(st.x - M);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         if (lane == 0) P.lse[si] = M + log2f(L);
     }
     // phase 1: (m, l) of every record, block max of m
@@ -346,7 +346,7 @@ constexpr int MERGE_B_THREADS = 1024;
 constexpr int MERGE_B_KEEP = 4;           // records per lane and round
 
 template <int HD>
-__global__ void __launch_bounds__(MERGE_B_THREADS) k_merge_balanced(const MergeParams P) {
+__device__ __forceinline__ void merge_balanced(const MergeParams& P) {
     constexpr int RS = HD + 4;                                   // floats per internal record
     constexpr int NWARP = MERGE_B_THREADS / 32, DPW = (HD / 4) / NWARP;   // float4 lanes per warp: 1 or 2
     static_assert(DPW >= 1 && DPW * NWARP * 4 == HD, "one float4 lane per warp and step");
@@ -521,6 +521,80 @@ __global__ void __launch_bounds__(MERGE_B_THREADS) k_merge_balanced(const MergeP
             }
         }
     }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(MERGE_B_THREADS) k_merge_balanced(const MergeParams P) { merge_balanced<HD>(P); }
+
+// The same merge for many (row, head) items of few records each, one warp per item: a batch cuts every (sequence, kv head)
+// into two or three pieces, and a block of 1024 threads per item then spends its time starting up (2048 items: 48 us; this
+// way 8 us).  Lane s holds the weight of record s, the lanes own the output's float4s; the records' loads are independent.
+// Items are numbered as the blocks of k_merge_balanced.
+constexpr int MERGE_M_THREADS = 256;
+template <int HD>
+__device__ __forceinline__ void merge_many(const MergeParams& P, int rowhead) {
+    constexpr int RS = HD + 4, Q4 = HD / 128;                    // float4s per lane
+    const int lane = threadIdx.x & 31;
+    const int hq = rowhead % P.Hq, rowidx = rowhead / P.Hq;
+    const int i = rowidx / P.rows, r = rowidx % P.rows;
+    const int kvh = hq / P.G, h = hq % P.G;
+    const int per = P.hdr[0], c0 = P.hdr[2 + i], nt = P.hdr[3 + i] - c0;
+    if (nt <= 0) return;                                         // inactive sequence: no output
+    int clo, chi;
+    fd::item_ctas(P.cph, per, P.Hkv, c0, nt, kvh, clo, chi);
+    const int RG = P.rows * P.G, count = chi - clo + 1;
+    const float* base = P.part + ((size_t)(clo + i * P.Hkv + kvh) * RG + r * P.G + h) * (size_t)RS;
+    const size_t stride = (size_t)RG * RS;
+    float M = NEG_BIG, L = 0.f;
+    float4 acc[Q4];
+#pragma unroll
+    for (int j = 0; j < Q4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < count; s0 += 32) {
+        const int ns = min(32, count - s0);
+        const float2 ml = lane < ns ? *reinterpret_cast<const float2*>(base + (s0 + lane) * stride + HD) : make_float2(NEG_BIG, 0.f);
+        float mx = ml.x;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float Mn = fmaxf(M, mx), sc = fast_exp2(M - Mn), w = fast_exp2(ml.x - Mn);
+        float ls = w * ml.y;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
+        L = fmaf(L, sc, ls);
+        M = Mn;
+#pragma unroll
+        for (int j = 0; j < Q4; ++j) { acc[j].x *= sc; acc[j].y *= sc; acc[j].z *= sc; acc[j].w *= sc; }
+#pragma unroll 4
+        for (int s = 0; s < ns; ++s) {
+            const float ws = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+            for (int j = 0; j < Q4; ++j) {
+                const float4 o = *reinterpret_cast<const float4*>(base + (s0 + s) * stride + 4 * (lane + 32 * j));
+                acc[j].x = fmaf(o.x, ws, acc[j].x); acc[j].y = fmaf(o.y, ws, acc[j].y);
+                acc[j].z = fmaf(o.z, ws, acc[j].z); acc[j].w = fmaf(o.w, ws, acc[j].w);
+            }
+        }
+    }
+    const float il = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int j = 0; j < Q4; ++j) {
+        const size_t oi = ((size_t)rowidx * P.Hq + hq) * HD + 4 * (lane + 32 * j);
+        if (P.out_f16) {
+            const __half2 a = __floats2half2_rn(acc[j].x * il, acc[j].y * il), b = __floats2half2_rn(acc[j].z * il, acc[j].w * il);
+            *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(P.out) + oi) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + oi) =
+                make_float4(acc[j].x * il, acc[j].y * il, acc[j].z * il, acc[j].w * il);
+        }
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_many(const MergeParams P) {
+    pdl_trigger();
+    pdl_wait();
+    const int item = blockIdx.x * (MERGE_M_THREADS / 32) + (threadIdx.x >> 5);
+    if (item < P.n_rows * P.Hq) merge_many<HD>(P, item);
 }
 
 // The receiving half of the exchange on its own: one block per (row, head) waits for every device's record of the

@@ -3,19 +3,20 @@
 // lse its log-sum-exp.  The attention kernels (VAR_TRACK) leave what is needed for lse, with denominators summed in fp32
 // from unrounded weights.
 //
-// k_track_step, one row per sequence: the decode kernel kept the scores (16 bytes per position and kv head at four heads,
-// beside the 272 bytes of K and V it streams), so the cache is not read again; a thread owns a position.
-// k_track_chunk, a prompt chunk: the scores are formed a second time, S^T = K Q^T with the keys on the MMA rows, so that a
-// thread holds all rows of its keys in turn and the sum over rows stays in its registers; only K is read.
+// track_step, one row per sequence: the decode kernel kept the scores (16 bytes per position and kv head at four heads,
+// beside the 272 bytes of K and V it streams), so the cache is not read again; it runs beside the merge of the split records,
+// in the same launch.
+// k_track_chunk, a prompt chunk: the scores are formed a second time; only K is read.
 #pragma once
 #include "common.cuh"
+#include "exact.cuh"
+#include "prefill.cuh"
 #include "work_cut.h"
 
 namespace battn {
 namespace tr {
 
 constexpr int TILE = 64;                    // tiles of the decode kernel's scores
-constexpr int STEP_THREADS = 256;
 
 struct StepParams {
     const int* hdr;          // the decode kernel's header, records and scores
@@ -28,57 +29,110 @@ struct StepParams {
     int n_seq, Hkv, G, HD, cph;
     size_t stride;
 };
+struct StepMerge {           // one launch: blocks below `merge_blocks` merge the outputs, the others accumulate the weights
+    MergeParams merge;
+    StepParams step;
+    int merge_blocks;
+};
 
-__global__ void __launch_bounds__(STEP_THREADS) k_track_step(const StepParams P) {
+// log-sum-exp of head `h` of an item over the records of the CTAs that hold a piece of it, by one warp
+__device__ __forceinline__ float item_lse(const StepParams& P, int item, int clo, int chi, int h, int lane) {
+    const float* rec = P.part + ((size_t)(clo + item) * P.G + h) * (P.HD + 4) + P.HD;
+    const size_t step = (size_t)P.G * (P.HD + 4);
+    float M = NEG_BIG, L = 0.f;
+    for (int s = lane; s <= chi - clo; s += 32) {
+        const float4 r = *reinterpret_cast<const float4*>(rec + s * step);     // m, rounded l, l
+        const float Mn = fmaxf(M, r.x);
+        L = L * fast_exp2(M - Mn) + r.z * fast_exp2(r.x - Mn);
+        M = Mn;
+    }
+    float Mx = M;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) Mx = fmaxf(Mx, __shfl_xor_sync(0xffffffffu, Mx, o));
+    L *= fast_exp2(M - Mx);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    return Mx + log2f(L);
+}
+
+// Block `cta` of `n_cta` accumulates its contiguous share of the scores' tiles, a thread per position, four in flight.
+template <int THREADS>
+__device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_cta) {
     extern __shared__ int s_cum[];                               // [n_seq + 1]
     __shared__ float s_lse[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_wait();
-    pdl_trigger();
-    for (int i = tid; i <= P.n_seq; i += STEP_THREADS) s_cum[i] = P.hdr[2 + i];
+    for (int i = tid; i <= P.n_seq; i += THREADS) s_cum[i] = P.hdr[2 + i];
     const int per_cta = P.hdr[0];
     __syncthreads();
     const int total = P.Hkv * s_cum[P.n_seq];
-    const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    const int g1 = min(total, ((int)blockIdx.x + 1) * share);
-    for (int g = blockIdx.x * share; g < g1;) {
+    const int share = (total + n_cta - 1) / n_cta;
+    const int g1 = min(total, (cta + 1) * share);
+    for (int g = cta * share; g < g1;) {
         const fd::Piece pc = fd::locate(g, g1, s_cum, P.n_seq, P.Hkv);
         const int c0 = s_cum[pc.i], nt = s_cum[pc.i + 1] - c0;
         const int p = P.pos[pc.i], slot = P.kslot ? P.kslot[pc.i] : 0;
-        // lse of every head of the group over the records of the CTAs that hold a piece of this item
         int clo, chi;
         fd::item_ctas(P.cph, per_cta, P.Hkv, c0, nt, pc.kvh, clo, chi);
-        __syncthreads();
+        __syncthreads();                                         // the previous piece has used s_lse
         if (warp < P.G) {
-            const float* rec = P.part + ((size_t)(clo + pc.i * P.Hkv + pc.kvh) * P.G + warp) * (P.HD + 4) + P.HD;
-            const size_t step = (size_t)P.G * (P.HD + 4);
-            float M = NEG_BIG, L = 0.f;
-            for (int s = lane; s <= chi - clo; s += 32) {
-                const float4 r = *reinterpret_cast<const float4*>(rec + s * step);     // m, rounded l, l
-                const float Mn = fmaxf(M, r.x);
-                L = L * fast_exp2(M - Mn) + r.z * fast_exp2(r.x - Mn);
-                M = Mn;
-            }
-            float Mx = M;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) Mx = fmaxf(Mx, __shfl_xor_sync(0xffffffffu, Mx, o));
-            L *= fast_exp2(M - Mx);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            if (lane == 0) s_lse[warp] = Mx + log2f(L);
+            const float lse = item_lse(P, pc.i * P.Hkv + pc.kvh, clo, chi, warp, lane);
+            if (lane == 0) s_lse[warp] = lse;
         }
         __syncthreads();
-        const size_t base = ((size_t)slot * P.Hkv + pc.kvh) * P.stride;
-        for (int k = tid; k < pc.n * TILE; k += STEP_THREADS) {
-            const int key = pc.tl * TILE + k;
-            if (key > p) break;
-            const float* sc = P.scores + ((size_t)g * TILE + k) * P.G;
-            float w = 0.f;
-            for (int h = 0; h < P.G; ++h) w += fast_exp2(sc[h] - s_lse[h]);
-            if (P.in && key < p) w += P.in[base + key];           // the call's own position starts from nothing
-            P.out[base + key] = w;
+        const int first = pc.tl * TILE, keys = min(pc.n * TILE, p + 1 - first);
+        const float* in = P.in ? P.in + ((size_t)slot * P.Hkv + pc.kvh) * P.stride + first : nullptr;
+        float* out = P.out + ((size_t)slot * P.Hkv + pc.kvh) * P.stride + first;
+        const float* sc = P.scores + (size_t)g * TILE * P.G;
+        constexpr int UN = 4;
+        if (P.G == 4) {                                          // the usual group: a position's scores are one 16-byte load
+            const float l0 = s_lse[0], l1 = s_lse[1], l2 = s_lse[2], l3 = s_lse[3];
+            for (int k0 = tid; k0 < keys; k0 += UN * THREADS) {
+                float4 v[UN];
+                float w[UN];
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int k = k0 + u * THREADS;
+                    v[u] = k < keys ? *reinterpret_cast<const float4*>(sc + 4 * (size_t)k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    w[u] = in && k < keys && first + k < p ? in[k] : 0.f;   // the call's own position starts from nothing
+                }
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int k = k0 + u * THREADS;
+                    if (k < keys)
+                        out[k] = ((fast_exp2(v[u].x - l0) + fast_exp2(v[u].y - l1)) + (fast_exp2(v[u].z - l2) + fast_exp2(v[u].w - l3))) + w[u];
+                }
+            }
+        } else {
+            for (int k = tid; k < keys; k += THREADS) {
+                float w = 0.f;
+                for (int h = 0; h < P.G; ++h) w += fast_exp2(sc[(size_t)k * P.G + h] - s_lse[h]);
+                out[k] = w + (in && first + k < p ? in[k] : 0.f);
+            }
         }
         g += pc.n;
+    }
+}
+
+// few items (one or two sequences): the merge is one latency chain, see k_merge_balanced
+template <int HD>
+__global__ void __launch_bounds__(MERGE_B_THREADS) k_merge_track_few(const StepMerge P) {
+    if ((int)blockIdx.x < P.merge_blocks) {
+        merge_balanced<HD>(P.merge);
+    } else {
+        pdl_trigger();
+        pdl_wait();
+        track_step<MERGE_B_THREADS>(P.step, (int)blockIdx.x - P.merge_blocks, (int)gridDim.x - P.merge_blocks);
+    }
+}
+template <int HD>
+__global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_track_many(const StepMerge P) {
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.x < P.merge_blocks) {
+        const int item = blockIdx.x * (MERGE_M_THREADS / 32) + (threadIdx.x >> 5);
+        if (item < P.merge.n_rows * P.merge.Hq) merge_many<HD>(P.merge, item);
+    } else {
+        track_step<MERGE_M_THREADS>(P.step, (int)blockIdx.x - P.merge_blocks, (int)gridDim.x - P.merge_blocks);
     }
 }
 
@@ -98,139 +152,299 @@ struct ChunkParams {
     Paging pg;
 };
 
-constexpr int CW = 8;                       // warps; each owns 16 keys of a 128-key tile
-constexpr int CTHREADS = CW * 32, CKEYS = 16 * CW;
-constexpr int CPAIRS = 64;                  // (row, head) pairs of a Q tile
+// ---- the weights of a prompt chunk -------------------------------------------------------------------------------------
+// Persistent CTAs, one per SM; a unit is (kv head, 256 keys at head_dim 128, 128 keys at 256).  S^T = K Q^T on tcgen05 with
+// 128 keys on the M side, so that a TMEM lane is a key and the sum over the rows is a sum over columns, inside one thread.
+//   * K is the tensor-memory A operand and stays there for the unit, in two exact fp16 parts like in the prompt kernels
+//     (hi = fp16(d x), lo = d x - hi): the scores carry no rounding of K.  From shared memory it would be read again by
+//     every product, and a 128-column product with both operands there runs into the shared-memory bandwidth.
+//   * Q tiles of 128 (row, head) pairs stream from L2 through a ring as the B operand; every one serves all keys of the unit
+//     (two M tiles at head_dim 128: half the L2 traffic, which at one would be near 7 TB/s).
+//   * Two accumulators of 128 columns; each of two groups of four warps empties its own: w += 2^(s c - lse), one exponential
+//     per score.  The exponentials (16 per cycle and SM) take as long as the two products: that balance is the bound.
+//   * Between units the eight warps convert the next K, whose raw records were fetched ahead.
+// Against the form with warp MMAs and scales applied to fp32 sums (512 rows at 32K, 8 kv heads): 705 -> 262 us.
+constexpr int QN = 128;                     // pairs per Q tile
+constexpr int CTHREADS = 14 * 32;           // warps 0-7 convert K and sum weights, 8-11 load Q, 12 issues the MMAs, 13 loads K
+constexpr int MAX_PAIRS = MAX_PREFILL * 8;
 
 template <int HD>
 struct ChunkCfg {
     static constexpr int NBLK = HD / 32, REC = HD + 2 * NBLK;
-    static constexpr int QSTR = HD + 32;                        // halves per staged Q row (as in flash_decode.cuh)
-    static constexpr int Q_BYTES = CPAIRS * QSTR * 2;
-    static constexpr int SMEM = 2 * Q_BYTES + 2 * CPAIRS * 8;   // two Q tiles, their (lse, position) pairs
+    static constexpr int KT = HD == 128 ? 2 : 1;                 // key tiles (M = 128) per unit
+    static constexpr int KEYS = 128 * KT;
+    static constexpr int Q_SUB = QN * 128;                       // one 64-dim sub-tile [128 pairs][128 B], 128-byte swizzle
+    static constexpr int Q_BYTES = (HD / 64) * Q_SUB;
+    static constexpr int QST = HD == 128 ? 4 : 2;                // Q ring
+    static constexpr int RAW = 128 * REC;                        // raw records of one key tile
+    static constexpr int OFF_RAW = QST * Q_BYTES;
+    static constexpr int OFF_LSE = OFF_RAW + KT * RAW;           // -lse of every pair of the unit's kv head
+    static constexpr int OFF_XCH = OFF_LSE + MAX_PAIRS * 4;
+    static constexpr int OFF_BAR = OFF_XCH + 128 * 4;
+    static constexpr int SMEM = OFF_BAR + 16 * 8 + 16 + 1024;    // + slack to align the base to 1024
+    static constexpr int T_LO = HD / 2;                          // columns from the high to the low part of a K tile
+    static constexpr int T_D = 256;                              // two accumulators of 128 columns
+    static_assert(KT * HD == 256 && SMEM <= 226 * 1024, "tensor and shared memory budget");
 };
+enum { B_RAWF = 0, B_RAWE = 1, B_KRDY = 2, B_QF = 3, B_QE = 7, B_DF = 11, B_DE = 13, N_CBARS = 15 };
 
-// One unit = (kv head, 128 keys).  The warp's 16 keys are the A operand of every product of the unit: the exact integers of
-// the records, kept in registers, with the block scales applied to the fp32 sums of each 32-dim block afterwards, so the
-// scores carry no rounding of K.  Q tiles of 64 pairs are double-buffered in shared memory.
 template <int HD>
-__global__ void __launch_bounds__(CTHREADS) k_track_chunk(const ChunkParams P) {
+__global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P) {
+    using namespace pf;
     using C = ChunkCfg<HD>;
-    constexpr int NBLK = C::NBLK, REC = C::REC, QSTR = C::QSTR;
-    extern __shared__ __align__(16) uint8_t smem[];
-    __half* s_q = reinterpret_cast<__half*>(smem);
-    float2* s_st = reinterpret_cast<float2*>(smem + 2 * C::Q_BYTES);       // (lse, last visible position as int bits)
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, t4 = lane & 3;
+    constexpr int NBLK = C::NBLK, REC = C::REC, KT = C::KT, QST = C::QST;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float* s_nl = reinterpret_cast<float*>(smem + C::OFF_LSE);
+    float* s_xch = reinterpret_cast<float*>(smem + C::OFF_XCH);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_BAR + 16 * 8);    // [0] tmem base, [1] abort
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_trigger();
     const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.rows, 0, 0, P.pstride, P.n_slots, P.status);
-    if (!sr.active) return;
-    const int n = sr.hi, pairs = P.rows * P.G, n_qt = (pairs + CPAIRS - 1) / CPAIRS;
-    const int tiles = (n + CKEYS - 1) / CKEYS, units = tiles * P.Hkv;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int kvh = u % P.Hkv, t0 = (u / P.Hkv) * CKEYS;
-        // ---- this thread's parts of the records of keys k0, k1 (MMA rows gid, gid + 8) --------------------------------
-        const int k0 = t0 + warp * 16 + gid, k1 = k0 + 8;
-        uint32_t a[NBLK][2][4];
-        float d0[NBLK], d1[NBLK];
+    const int n = sr.hi, p0 = sr.p0, G = P.G;
+    const int pairs = P.rows * G, n_qt = (pairs + QN - 1) / QN;
+    const int units = sr.active ? (n + C::KEYS - 1) / C::KEYS * P.Hkv : 0;
+    if ((int)blockIdx.x >= units) return;
+    if (tid == 0) {
+        mbar_init(&bars[B_RAWF], 1); mbar_init(&bars[B_RAWE], 8); mbar_init(&bars[B_KRDY], 8);
+        for (int i = 0; i < QST; ++i) { mbar_init(&bars[B_QF + i], 4); mbar_init(&bars[B_QE + i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_DF + i], 1); mbar_init(&bars[B_DE + i], 4); }
+        misc[1] = 0;
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(const_cast<uint32_t*>(&misc[0]))), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = misc[0];
+    // bounded wait that degrades to "do not wait" once any wait has run out
+    auto wait = [&](int b, uint32_t parity) {
+        if (mbar_try_wait(&bars[b], parity)) return;
+        if (misc[1]) return;
+        if (!mbar_wait_backoff(&bars[b], parity, 20)) {
+            atomicOr(P.status, BATTN_DEV_WAIT_TIMEOUT);
+            misc[1] = 1;
+        }
+    };
+    // unit u: keys t0 .. of kv head kvh; rows before Q tile qt0 see none of them
+    auto unit_t0 = [&](int u) { return u / P.Hkv * C::KEYS; };
+    auto unit_qt0 = [&](int t0) { return max(0, t0 - p0) * G / QN; };
+    auto unit_tiles = [&](int t0) { return KT == 1 || t0 + 128 >= n ? 1 : KT; };
+
+    if (warp < 8) {
+        // ======================= K operand, then the weights: one thread per key and accumulator ====================
+        const int grp = warp >> 2, row = tid & 127;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t used = 0, steps = 0, unit = 0;                  // accumulators emptied by this group, products so far, units
+        for (int u = blockIdx.x; u < units; u += gridDim.x, ++unit) {
+            const int kvh = u % P.Hkv, t0 = unit_t0(u), qt0 = unit_qt0(t0);
+            // every product of the previous unit has completed (each group has seen its last one), s_nl and s_xch are read
+            named_bar_sync(1, 256);
+            for (int i = tid; i < n_qt * QN; i += 256) {
+                const int r = i / G;
+                s_nl[i] = i < pairs ? -P.lse[(size_t)r * P.Hq + kvh * G + (i - r * G)] : NEG_BIG;      // no pair: weight 0
+            }
+            wait(B_RAWF, unit & 1);
+            if (KT == 1 || grp < unit_tiles(t0)) {
+                // head_dim 128: the group's key tile; 256: its half of the dims of the one tile
+                const uint8_t* rec = smem + C::OFF_RAW + (KT == 2 ? grp * C::RAW : 0) + row * REC;
+                const int d0 = KT == 2 ? 0 : 128 * grp;
+                const uint32_t tk = tmem + lane_base + (KT == 2 ? grp * HD : 0) + d0 / 2;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t hi[32], lo[32];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int key = e ? k1 : k0;
-            const bool in = key < n;
-            const uint8_t* rec = P.kvk;
-            if (in) rec += kv_rec_index(P.pg, sr.slot, kvh, P.Hkv, P.pstride, key, P.status) * (size_t)REC;
+                    for (int c = 0; c < 8; ++c) {                // 8 dims each
+                        const int d = d0 + 64 * half + 8 * c;
+                        const __half2 s2 = __half2half2(reinterpret_cast<const __half*>(rec)[d >> 5]);
+                        const uint32_t su = *reinterpret_cast<const uint32_t*>(&s2);
+                        const uint2 w = *reinterpret_cast<const uint2*>(rec + 2 * NBLK + d);
+                        const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+                        const uint32_t v[4] = {sub1152(widen_lo(x)), sub1152(widen_hi(x)), sub1152(widen_lo(y)), sub1152(widen_hi(y))};
 #pragma unroll
-            for (int b = 0; b < NBLK; ++b) {
-                const float d = in ? __half2float(reinterpret_cast<const __half*>(rec)[b]) : 0.f;
-                if (e) d1[b] = d; else d0[b] = d;
-                const uint2 w = in ? *reinterpret_cast<const uint2*>(rec + 2 * NBLK + b * 32 + t4 * 8) : make_uint2(0u, 0u);
-                const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
-                a[b][0][e] = sub1152(widen_lo(x)); a[b][0][2 + e] = sub1152(widen_hi(x));
-                a[b][1][e] = sub1152(widen_lo(y)); a[b][1][2 + e] = sub1152(widen_hi(y));
+                        for (int e = 0; e < 4; ++e) {
+                            hi[4 * c + e] = hmul2_u32(v[e], su);
+                            lo[4 * c + e] = hfma2_residual(v[e], su, hi[4 * c + e]);
+                        }
+                    }
+                    tmem_st32(tk + 32 * half, hi);
+                    tmem_st32(tk + C::T_LO + 32 * half, lo);
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&bars[B_RAWE]); mbar_arrive(&bars[B_KRDY]); }
+            named_bar_sync(1, 256);                              // s_nl is complete
+            const int key = t0 + (KT == 2 ? 128 * grp : 0) + row;
+            const bool mine = KT == 1 || grp < unit_tiles(t0);
+            const uint32_t tD = tmem + lane_base + C::T_D + grp * 128;
+            const uint64_t c2p = pack_f2(P.scale_log2, P.scale_log2);
+            float w0 = 0.f, w1 = 0.f;
+            for (int qt = qt0; qt < n_qt; ++qt, ++steps) {
+                if (KT == 2 ? !mine : (int)(steps & 1) != grp) continue;
+                wait(B_DF + grp, used & 1);
+                ++used;
+                tc_fence_after();
+                // pairs of this tile that see the key: index at least (key - p0) G
+                const int first = (key - p0) * G - qt * QN;
+                const bool masked = t0 + C::KEYS - 1 > p0 + qt * QN / G;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[64];
+                    tmem_ld32_nowait(tD + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                    tmem_ld32_nowait(tD + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+                    tmem_ld_wait();
+                    if (h == 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars[B_DE + grp]);
+                    }
+                    const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(s_nl + qt * QN + 64 * h);
+                    if (!masked) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const ulonglong2 l = nl[i];
+                            float e0, e1, e2, e3;
+                            ffma2(e0, e1, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
+                            ffma2(e2, e3, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
+                            w0 += fast_exp2(e0) + fast_exp2(e1);
+                            w1 += fast_exp2(e2) + fast_exp2(e3);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const ulonglong2 l = nl[i];
+                            float e[4];
+                            ffma2(e[0], e[1], __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
+                            ffma2(e[2], e[3], __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w0 += 64 * h + 4 * i + k >= first ? fast_exp2(e[k]) : 0.f;
+                        }
+                    }
+                }
+            }
+            float w = w0 + w1;
+            if (KT == 1) {                                       // the two groups share the keys
+                if (grp == 1) s_xch[row] = w;
+                named_bar_sync(1, 256);
+                if (grp == 0) w += s_xch[row];
+            }
+            if ((KT == 2 ? mine : grp == 0) && key < n) {
+                const size_t at = ((size_t)sr.slot * P.Hkv + kvh) * P.pstride + key;
+                if (P.in && key < p0) w += P.in[at];             // the call's own positions start from nothing
+                P.out[at] = w;
             }
         }
-        float w0 = 0.f, w1 = 0.f;
-        // rows before qt0 see none of these keys
-        const int qt0 = max(0, t0 - sr.p0) * P.G / CPAIRS;
-        auto load = [&](int qt, int buf) {
-            for (int idx = tid; idx < CPAIRS * (HD / 8); idx += CTHREADS) {
-                const int pr = idx / (HD / 8), ch = idx - pr * (HD / 8), pair = qt * CPAIRS + pr;
-                __half* dst = s_q + buf * (C::Q_BYTES / 2) + pr * QSTR + ch * 8;
+    } else if (warp < 12) {
+        // ======================= Q tiles: [pair][dim], 64-dim sub-tiles, 128-byte swizzle ================================
+        const int t = tid - 256;
+        uint32_t cnt = 0;
+        auto load = [&](int kvh, int qt, uint32_t c) {
+            uint8_t* dst = smem + (c % QST) * C::Q_BYTES;
+#pragma unroll 4
+            for (int idx = t; idx < QN * (HD / 8); idx += 128) {
+                const int pr = idx / (HD / 8), ch = idx - pr * (HD / 8), pair = qt * QN + pr;
+                uint8_t* to = dst + (ch >> 3) * C::Q_SUB + sw128(pr, ch & 7);
                 if (pair < pairs) {
-                    const int r = pair / P.G, h = pair - r * P.G;
-                    const size_t qi = ((size_t)r * P.Hq + kvh * P.G + h) * HD + ch * 8;
+                    const int r = pair / G;
+                    const size_t qi = ((size_t)r * P.Hq + kvh * G + (pair - r * G)) * HD + ch * 8;
                     if (P.q_f16) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)),
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)),
                                      "l"(reinterpret_cast<const __half*>(P.q) + qi) : "memory");
                     } else {
                         const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + qi);
                         const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + qi + 4);
-                        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_h2(x.x, x.y), pack_h2(x.z, x.w), pack_h2(y.x, y.y), pack_h2(y.z, y.w));
+                        *reinterpret_cast<uint4*>(to) = make_uint4(pack_h2(x.x, x.y), pack_h2(x.z, x.w), pack_h2(y.x, y.y), pack_h2(y.z, y.w));
                     }
                 } else {
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
                 }
-            }
-            if (tid < CPAIRS) {
-                const int pair = qt * CPAIRS + tid, r = pair / P.G, h = pair - r * P.G;
-                s_st[buf * CPAIRS + tid] = pair < pairs ? make_float2(P.lse[(size_t)r * P.Hq + kvh * P.G + h], __int_as_float(sr.p0 + r))
-                                                        : make_float2(0.f, __int_as_float(-1));
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        __syncthreads();                                        // the previous unit's tiles have been used
-        load(qt0, qt0 & 1);
-        for (int qt = qt0; qt < n_qt; ++qt) {
-            const int buf = qt & 1;
-            if (qt + 1 < n_qt) load(qt + 1, buf ^ 1);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncthreads();
-            const __half* qs = s_q + buf * (C::Q_BYTES / 2);
-            const bool masked = t0 + CKEYS - 1 > sr.p0 + qt * CPAIRS / P.G || (qt + 1) * CPAIRS > pairs;
-#pragma unroll 2
-            for (int nt = 0; nt < CPAIRS / 8; ++nt) {
-                float sv[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int b = 0; b < NBLK; ++b) {
-                    const uint4 qv = *reinterpret_cast<const uint4*>(qs + (nt * 8 + gid) * QSTR + b * 32 + t4 * 8);
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816(acc, a[b][0], qv.x, qv.y);
-                    mma16816(acc, a[b][1], qv.z, qv.w);
-                    sv[0] = fmaf(d0[b], acc[0], sv[0]);
-                    sv[1] = fmaf(d0[b], acc[1], sv[1]);
-                    sv[2] = fmaf(d1[b], acc[2], sv[2]);
-                    sv[3] = fmaf(d1[b], acc[3], sv[3]);
+        auto publish = [&](uint32_t c) {                         // tile c has landed: hand it to the tensor core's proxy
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[B_QF + c % QST]);
+        };
+        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+            const int t0 = unit_t0(u);
+            for (int qt = unit_qt0(t0); qt < n_qt; ++qt, ++cnt) {
+                if (QST == 2 && cnt > 0) {                       // a ring of two: the tile before must go first
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    publish(cnt - 1);
                 }
-                // columns 2 t4, 2 t4 + 1: their (lse, position) are neighbours
-                const float4 st = *reinterpret_cast<const float4*>(&s_st[buf * CPAIRS + nt * 8 + 2 * t4]);
-                float e0 = fast_exp2(fmaf(sv[0], P.scale_log2, -st.x)), e1 = fast_exp2(fmaf(sv[1], P.scale_log2, -st.z));
-                float e2 = fast_exp2(fmaf(sv[2], P.scale_log2, -st.x)), e3 = fast_exp2(fmaf(sv[3], P.scale_log2, -st.z));
-                if (masked) {
-                    const int l0 = __float_as_int(st.y), l1 = __float_as_int(st.w);
-                    if (k0 > l0) e0 = 0.f;
-                    if (k0 > l1) e1 = 0.f;
-                    if (k1 > l0) e2 = 0.f;
-                    if (k1 > l1) e3 = 0.f;
+                if (cnt >= QST) wait(B_QE + cnt % QST, (cnt / QST - 1) & 1);
+                load(u % P.Hkv, qt, cnt);
+                if (QST > 2 && cnt > 0) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    publish(cnt - 1);
                 }
-                w0 += e0 + e1;
-                w1 += e2 + e3;
             }
-            __syncthreads();                                    // the buffer is refilled next
         }
-        w0 += __shfl_xor_sync(0xffffffffu, w0, 1); w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-        w1 += __shfl_xor_sync(0xffffffffu, w1, 1); w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
-        if (t4 < 2) {
-            const int key = t4 ? k1 : k0;
-            if (key < n) {
-                const size_t at = ((size_t)sr.slot * P.Hkv + kvh) * P.pstride + key;
-                float w = t4 ? w1 : w0;
-                if (P.in && key < sr.p0) w += P.in[at];
-                P.out[at] = w;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        publish(cnt - 1);
+    } else if (warp == 12) {
+        // ======================= the products ============================================================================
+        if (lane == 0) {
+            const uint32_t id = umma_idesc(128, QN);
+            const uint64_t qd0 = umma_desc(smem_u32(smem));
+            uint32_t cnt = 0, unit = 0, filled[2] = {0, 0};
+            for (int u = blockIdx.x; u < units; u += gridDim.x, ++unit) {
+                const int t0 = unit_t0(u), tiles = unit_tiles(t0);
+                wait(B_KRDY, unit & 1);
+                for (int qt = unit_qt0(t0); qt < n_qt; ++qt, ++cnt) {
+                    wait(B_QF + cnt % QST, (cnt / QST) & 1);
+                    const uint64_t qd = qd0 + (uint64_t)((cnt % QST) * (C::Q_BYTES >> 4));
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        if (kt >= tiles) break;
+                        const int b = KT == 2 ? kt : (int)(cnt & 1);
+                        const uint32_t f = b ? filled[1] : filled[0];
+                        if (f > 0) wait(B_DE + b, (f - 1) & 1);
+                        tc_fence_after();
+                        const uint32_t d = tmem + C::T_D + b * 128, ka = tmem + kt * HD;
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int ks = 0; ks < HD / 16; ++ks)
+                                umma_f16_ts(d, ka + part * C::T_LO + 8 * ks, qd + (uint64_t)((ks >> 2) * (C::Q_SUB >> 4) + 2 * (ks & 3)),
+                                            id, part > 0 || ks > 0);
+                        umma_commit(&bars[B_DF + b]);
+                        if (b) ++filled[1]; else ++filled[0];
+                    }
+                    umma_commit(&bars[B_QE + cnt % QST]);
+                }
+            }
+        }
+    } else if (lane == 0) {
+        // ======================= raw K records, one unit ahead ================================================================
+        uint32_t unit = 0;
+        for (int u = blockIdx.x; u < units; u += gridDim.x, ++unit) {
+            const int kvh = u % P.Hkv, t0 = unit_t0(u), tiles = unit_tiles(t0);
+            if (unit > 0) wait(B_RAWE, (unit - 1) & 1);
+            uint32_t bytes = 0;
+            for (int kt = 0; kt < tiles; ++kt) bytes += (uint32_t)min(128, P.pstride - t0 - 128 * kt) * REC;
+            mbar_expect_tx(&bars[B_RAWF], bytes);
+            for (int kt = 0; kt < tiles; ++kt) {
+                const int key = t0 + 128 * kt;
+                bulk_g2s(smem + C::OFF_RAW + kt * C::RAW, P.kvk + kv_rec_index(P.pg, sr.slot, kvh, P.Hkv, P.pstride, key, P.status) * (size_t)REC,
+                         (uint32_t)min(128, P.pstride - key) * REC, &bars[B_RAWF]);
             }
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
 }
 
 }  // namespace tr

@@ -52,27 +52,26 @@ def quantised(g, k, v):
 
 
 def weights64(g, q, krec, p0: int, n_sink: int | None = None, window: int | None = None):
-    """Softmax weights [n_head][rows][keys] in float64 of rows at p0 ...: causal, with `window` also windowed with sinks."""
+    """Softmax weights [n_head][rows][keys] in float64 (torch, on the GPU) of rows at p0 ...: causal, with `window` also windowed with sinks."""
     rows, n = q.shape[0], p0 + q.shape[0]
-    kd = values(krec[:, :n], g.head_dim)
-    qd = q.astype(np.float64)
+    kd = torch.from_numpy(values(krec[:, :n], g.head_dim)).cuda()
+    qd = torch.from_numpy(q.astype(np.float64)).cuda().reshape(rows, g.n_kv, g.group, -1)
     scale = g.softmax_scale or g.head_dim ** -0.5
-    a = np.einsum("rhd,hnd->hrn", qd, np.repeat(kd, g.group, axis=0)) * scale
-    key, at = np.arange(n)[None], (p0 + np.arange(rows))[:, None]
+    a = torch.einsum("rhgd,hnd->hgrn", qd, kd).reshape(g.n_head, rows, n) * scale
+    key, at = torch.arange(n, device="cuda")[None], (p0 + torch.arange(rows, device="cuda"))[:, None]
     see = key <= at
     if window is not None:
         see &= (key > at - window) | (key < n_sink)
-    a = np.where(see[None], a, -np.inf)
-    w = np.exp(a - a.max(-1, keepdims=True))
-    return w / w.sum(-1, keepdims=True)
+    a = torch.where(see[None], a, -torch.inf)
+    w = torch.exp(a - a.amax(-1, keepdim=True))
+    return w / w.sum(-1, keepdim=True)
 
 
 def attend64(g, q, krec, vrec, p0, n_sink=None, window=None):
-    w = weights64(g, q, krec, p0, n_sink, window)
-    vd = np.repeat(values(vrec[:, :p0 + q.shape[0]], g.head_dim), g.group, axis=0)
-    # a hidden position may hold anything: its weight is zero and it is left out
-    seen = (w > 0).any((0, 1))
-    return np.einsum("hrn,hnd->rhd", w[:, :, seen], vd[:, seen])
+    rows, n = q.shape[0], p0 + q.shape[0]
+    w = weights64(g, q, krec, p0, n_sink, window).reshape(g.n_kv, g.group * rows, n)
+    o = w @ torch.from_numpy(values(vrec[:, :n], g.head_dim)).cuda()
+    return o.reshape(g.n_head, rows, -1).transpose(0, 1).cpu().numpy()
 
 
 U = 2.0 ** -11        # half a step of fp16
@@ -154,7 +153,7 @@ def evict_list(score: np.ndarray, budget: int, n_sink: int, n_recent: int) -> np
 
 def score64(g, q, krec, p0: int, score_in):
     """Accumulated weights [n_kv][p0 + rows] in float64."""
-    s = weights64(g, q, krec, p0).sum(1).reshape(g.n_kv, g.group, -1).sum(1)
+    s = weights64(g, q, krec, p0).sum(1).reshape(g.n_kv, g.group, -1).sum(1).cpu().numpy()
     if score_in is not None:
         s[:, :p0] += score_in[:, :p0]
     return s
@@ -169,8 +168,9 @@ def assert_scores(got, want, g, q, krec, p0, what=""):
     weight at most rows * group: each addition is off by 2^-24 of a sum of positive terms.  ex2.approx is off by 2^-22, twice
     per weight and once per merge level: 8 * 2^-22.  The accumulated value adds one rounding."""
     n = krec.shape[1]
-    kd = np.abs(values(krec, g.head_dim))
-    a = np.einsum("rhd,hnd->hrn", np.abs(q.astype(np.float64)), np.repeat(kd, g.group, axis=0)).max()
+    kd = torch.from_numpy(values(krec, g.head_dim)).cuda().abs()
+    qd = torch.from_numpy(q.astype(np.float64)).cuda().abs().reshape(q.shape[0], g.n_kv, g.group, -1)
+    a = float(torch.einsum("rhgd,hnd->hgrn", qd, kd).max())
     a *= (g.softmax_scale or g.head_dim ** -0.5) * 1.4427
     rel = 2 * 0.6932 * 16 * 2.0 ** -23 * a + 8 * 2.0 ** -22 + (n / 2 + q.shape[0] * g.group) * 2.0 ** -24
     off = np.abs(np.asarray(got, dtype=np.float64) - want)
