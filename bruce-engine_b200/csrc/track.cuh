@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
     pdl_wait();
     pdl_trigger();
     const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.rows, 0, 0, P.pstride, P.n_slots, P.status);
-    const int n = sr.hi, p0 = sr.p0, G = P.G;
+    const int n = sr.hi, p0 = sr.p0, G = P.G, lg = __ffs(G) - 1;         // the group divides 128: a power of two
     const int pairs = P.rows * G, n_qt = (pairs + QN - 1) / QN;
     const int units = sr.active ? (n + C::KEYS - 1) / C::KEYS * P.Hkv : 0;
     if ((int)blockIdx.x >= units) return;
@@ -246,10 +246,6 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
             const int kvh = u % P.Hkv, t0 = unit_t0(u), qt0 = unit_qt0(t0);
             // every product of the previous unit has completed (each group has seen its last one), s_nl and s_xch are read
             named_bar_sync(1, 256);
-            for (int i = tid; i < n_qt * QN; i += 256) {
-                const int r = i / G;
-                s_nl[i] = i < pairs ? -P.lse[(size_t)r * P.Hq + kvh * G + (i - r * G)] : NEG_BIG;      // no pair: weight 0
-            }
             wait(B_RAWF, unit & 1);
             if (KT == 1 || grp < unit_tiles(t0)) {
                 // head_dim 128: the group's key tile; 256: its half of the dims of the one tile
@@ -281,7 +277,10 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
             tc_fence_before();
             __syncwarp();
             if (lane == 0) { mbar_arrive(&bars[B_RAWE]); mbar_arrive(&bars[B_KRDY]); }
-            named_bar_sync(1, 256);                              // s_nl is complete
+            // -lse of every pair, while the first products run
+            for (int i = tid + qt0 * QN; i < n_qt * QN; i += 256)
+                s_nl[i] = i < pairs ? -P.lse[(size_t)(i >> lg) * P.Hq + kvh * G + (i & (G - 1))] : NEG_BIG;    // no pair: weight 0
+            named_bar_sync(1, 256);
             const int key = t0 + (KT == 2 ? 128 * grp : 0) + row;
             const bool mine = KT == 1 || grp < unit_tiles(t0);
             const uint32_t tD = tmem + lane_base + C::T_D + grp * 128;
@@ -347,14 +346,16 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
         const int t = tid - 256;
         uint32_t cnt = 0;
         auto load = [&](int kvh, int qt, uint32_t c) {
-            uint8_t* dst = smem + (c % QST) * C::Q_BYTES;
-#pragma unroll 4
-            for (int idx = t; idx < QN * (HD / 8); idx += 128) {
-                const int pr = idx / (HD / 8), ch = idx - pr * (HD / 8), pair = qt * QN + pr;
-                uint8_t* to = dst + (ch >> 3) * C::Q_SUB + sw128(pr, ch & 7);
+            // thread t: 16-byte chunk `ch` of every PSTEP-th pair
+            constexpr int PSTEP = 128 / (HD / 8);
+            const int ch = t & (HD / 8 - 1), pr0 = t / (HD / 8);
+            uint8_t* dst = smem + (c % QST) * C::Q_BYTES + (ch >> 3) * C::Q_SUB;
+#pragma unroll 8
+            for (int pr = pr0; pr < QN; pr += PSTEP) {
+                const int pair = qt * QN + pr;
+                uint8_t* to = dst + sw128(pr, ch & 7);
                 if (pair < pairs) {
-                    const int r = pair / G;
-                    const size_t qi = ((size_t)r * P.Hq + kvh * G + (pair - r * G)) * HD + ch * 8;
+                    const size_t qi = ((size_t)(pair >> lg) * P.Hq + kvh * G + (pair & (G - 1))) * HD + ch * 8;
                     if (P.q_f16) {
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)),
                                      "l"(reinterpret_cast<const __half*>(P.q) + qi) : "memory");
