@@ -104,8 +104,9 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     }
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_TRACK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(tr::k_track_chunk<HD>, tr::ChunkCfg<HD>::SMEM)) != cudaSuccess) return e;
-    if ((e = allow_smem(ev::k_evict_select, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
-    if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::SMEM)) != cudaSuccess) return e;
+    if ((e = allow_smem(ev::k_evict_select<1024>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
+    if ((e = allow_smem(ev::k_evict_select<512>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
+    if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::ROUND_MAX * ev::MoveCfg<HD>::PER)) != cudaSuccess) return e;
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 2, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
@@ -1162,15 +1163,22 @@ static int evict_impl(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score,
     while (c < ev::MAX_CLUSTER && n_seq * g.Hkv * c * 2 <= h->num_sms && c * ev::KEYS_PER_CTA < P.pstride) c *= 2;
     P.cluster = attr[0].val.clusterDim.x = c;
     P.keys = std::min(ev::KEYS_SMEM, (std::max(ev::KEYS_PER_CTA, (P.pstride + c - 1) / c) + 3) & ~3);
-    cfg.gridDim = dim3(n_seq * c, g.Hkv); cfg.blockDim = dim3(ev::SEL_THREADS); cfg.dynamicSmemBytes = (size_t)P.keys * 4;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, ev::k_evict_select, P);
+    const bool many = n_seq * g.Hkv > h->num_sms;
+    cfg.gridDim = dim3(n_seq * c, g.Hkv); cfg.blockDim = dim3(many ? 512 : 1024); cfg.dynamicSmemBytes = (size_t)P.keys * 4;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, many ? ev::k_evict_select<512> : ev::k_evict_select<1024>, P);
     if (e != cudaSuccess) return cuda_fail(h, e);
     // move: as many CTAs as a budget has rounds, so that a batch spreads evenly too
-    const int round = g.HD == 128 ? ev::MoveCfg<128>::ROUND : ev::MoveCfg<256>::ROUND;
+    int round = g.HD == 128 ? ev::MoveCfg<128>::ROUND : ev::MoveCfg<256>::ROUND;
+    const int round_max = g.HD == 128 ? ev::MoveCfg<128>::ROUND_MAX : ev::MoveCfg<256>::ROUND_MAX;
+    const int slot_bytes = g.HD == 128 ? ev::MoveCfg<128>::PER : ev::MoveCfg<256>::PER;
     for (c = 1; c < ev::MAX_CLUSTER && c * round < budget; ) c *= 2;
+    if (n_seq * g.Hkv * 2 * c <= h->num_sms) round = std::min(std::max(round, ((budget + c - 1) / c + 7) & ~7), round_max);
+    const bool one = c * round >= budget;
+    if (!one && 2 * round > round_max) round = round_max / 2 & ~7;
+    P.round = round;
     P.cluster = attr[0].val.clusterDim.x = c;
     cfg.gridDim = dim3(n_seq * c, g.Hkv, 2); cfg.blockDim = dim3(ev::MOVE_THREADS);
-    cfg.dynamicSmemBytes = g.HD == 128 ? ev::MoveCfg<128>::SMEM : ev::MoveCfg<256>::SMEM;
+    cfg.dynamicSmemBytes = (size_t)(one ? 1 : 2) * round * slot_bytes;
     e = g.HD == 128 ? cudaLaunchKernelEx(&cfg, ev::k_evict_move<128>, P) : cudaLaunchKernelEx(&cfg, ev::k_evict_move<256>, P);
     h->launches += 2;
     if (e == cudaSuccess) e = cudaGetLastError();

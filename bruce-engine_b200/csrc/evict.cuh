@@ -15,7 +15,7 @@ namespace battn {
 namespace ev {
 
 constexpr int MAX_CLUSTER = 8;              // the portable limit
-constexpr int SEL_THREADS = 1024, MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 256;
 constexpr int KEYS_SMEM = 40 * 1024;        // keys a CTA keeps in shared memory at most (160 KB); a longer share re-reads the rest
 // Candidates that are worth another CTA of the cluster: up to here a pass over them is shorter than the cluster barriers
 // (4160 positions, one CTA of eight: 23 -> 12 us)
@@ -36,6 +36,7 @@ struct Params {
     int Hkv, pstride, n_slots;
     int cluster;         // CTAs per cluster of this launch
     int keys;            // k_evict_select: keys its shared memory holds
+    int round;           // k_evict_move: records of a CTA in a round
     int* status;
     Paging pg;
 };
@@ -48,7 +49,8 @@ template <int N>
 __device__ __forceinline__ void load_rank(const uint32_t* p, int r, uint32_t (&v)[N]) {
     uint32_t ra;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(p)), "r"(r));
-    if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(ra) : "memory");
+    if constexpr (N == 4) asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(ra) : "memory");
+    else if constexpr (N == 2) asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(ra) : "memory");
     else                  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[0]) : "r"(ra) : "memory");
 }
 
@@ -60,6 +62,7 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 
 // Block-wide exclusive scan of one value per thread; `total` is the block's sum.
+template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp, uint32_t& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t x = v;
@@ -71,7 +74,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp, uin
     __syncthreads();                                 // the previous scan's sums have been read
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    uint32_t w = s_warp[lane];                       // 32 warps
+    uint32_t w = lane < THREADS / 32 ? s_warp[lane] : 0u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t t = __shfl_up_sync(0xffffffffu, w, o);
@@ -85,10 +88,10 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp, uin
 // One pass of the descent over BITS bits at SHIFT.  `hist` holds this CTA's counts of the keys that match the prefix so
 // far; every CTA adds up the cluster's counts itself and finds the same bin.  Counts of the CTAs before this one are kept
 // too: above the bin they end up in `gt_low`, in the last pass the bin's own are `eq_low`.
-template <int SHIFT, int BITS>
+template <int THREADS, int SHIFT, int BITS>
 __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_t* s_warp, volatile uint32_t* s_found,
                                         uint32_t& prefix, uint32_t& need, uint32_t& gt_low, uint32_t& eq_low) {
-    constexpr int PER = (1 << BITS) / SEL_THREADS;               // bins per thread, from the highest down
+    constexpr int PER = (1 << BITS) / THREADS;                   // bins per thread, from the highest down
     const int top = (1 << BITS) - PER * ((int)threadIdx.x + 1);  // lowest of this thread's bins
     uint32_t c[PER], low[PER];
 #pragma unroll
@@ -111,7 +114,7 @@ __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_
     uint32_t sum = 0, tot;
 #pragma unroll
     for (int e = 0; e < PER; ++e) sum += c[e];
-    uint32_t before = block_scan(sum, s_warp, tot);
+    uint32_t before = block_scan<THREADS>(sum, s_warp, tot);
 #pragma unroll
     for (int e = PER - 1; e >= 0; --e) {
         if (before < need && before + c[e] >= need) { s_found[0] = top + e; s_found[1] = before; }
@@ -128,9 +131,12 @@ __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_
     need -= s_found[1];
 }
 
-__global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P) {
+// SEL_THREADS: 1024 for few clusters, where a pass over the keys is the time; 512 once they outnumber the SMs, so that three
+// CTAs share one (32 sequences of up to 8192: 20 -> 13 us)
+template <int SEL_THREADS>
+__global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_select(const Params P) {
     extern __shared__ uint32_t s_key[];              // P.keys keys of this CTA's share
-    __shared__ __align__(8) uint32_t s_hist[2048 + 2048 + 1024];
+    __shared__ __align__(16) uint32_t s_hist[2048 + 2048 + 1024];
     __shared__ uint32_t s_warp[32], s_found[3][2], s_low[2];
     __shared__ int s_clash;
     const int CL = P.cluster, rank = (int)blockIdx.x % CL;
@@ -194,17 +200,17 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
     }
     // ---- the m-th best key ------------------------------------------------------------------------------------------------
     uint32_t T = 0, need = (uint32_t)m, gt_low = 0, eq_low = 0;
-    descend<21, 11>(s_hist, C, rank, s_warp, s_found[0], T, need, gt_low, eq_low);
+    descend<SEL_THREADS, 21, 11>(s_hist, C, rank, s_warp, s_found[0], T, need, gt_low, eq_low);
     for (int j = tid; j < len; j += SEL_THREADS) {
         const uint32_t k = key(j);
         if ((k >> 21) == T) atomicAdd(&s_hist[2048 + ((k >> 10) & 2047)], 1u);
     }
-    descend<10, 11>(s_hist + 2048, C, rank, s_warp, s_found[1], T, need, gt_low, eq_low);
+    descend<SEL_THREADS, 10, 11>(s_hist + 2048, C, rank, s_warp, s_found[1], T, need, gt_low, eq_low);
     for (int j = tid; j < len; j += SEL_THREADS) {
         const uint32_t k = key(j);
         if ((k >> 10) == T) atomicAdd(&s_hist[4096 + (k & 1023)], 1u);
     }
-    descend<0, 10>(s_hist + 4096, C, rank, s_warp, s_found[2], T, need, gt_low, eq_low);
+    descend<SEL_THREADS, 0, 10>(s_hist + 4096, C, rank, s_warp, s_found[2], T, need, gt_low, eq_low);
     if (C > 1) cluster_arrive();                                 // this CTA reads no other's counts any more
     // ---- better than the m-th, or equal and among the first `need` equal ones: the list, in order -----------------------
     uint32_t gt0 = 0, eq0 = 0;
@@ -225,7 +231,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
             if (j0 + e < len) mine += (k[e] > T ? 0x10000u : 0u) + (k[e] == T ? 1u : 0u);
         }
         uint32_t tot;
-        const uint32_t at = block_scan(mine, s_warp, tot);
+        const uint32_t at = block_scan<SEL_THREADS>(mine, s_warp, tot);
         uint32_t g = gt0 + (at >> 16), q = eq0 + (at & 0xFFFFu);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -238,13 +244,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) k_evict_select(const Params P)
     if (C > 1) cluster_wait();                       // the others have read this CTA's counts
 }
 
+// A round of a CTA: P.round records, chosen by the host: all of the CTA's part in one round when there are few clusters (the
+// SM has the room, and a round costs two trips to memory one after the other: 4096 records of 272 bytes, 15 -> 9 us),
+// otherwise 34 KB, so that several CTAs share an SM.  Two buffers when there is more than one round.
 template <int HD>
 struct MoveCfg {
     static constexpr int REC = HD + HD / 16, WORDS = REC / 8;
-    static constexpr int ROUND = HD == 128 ? 256 : 128;          // records of a CTA in a round (34 KB), two rounds in flight
-    static constexpr int BUF = ROUND * (REC + 4);                // records and scores
-    static constexpr int SMEM = 2 * BUF;
-    static_assert(ROUND * REC % 16 == 0 && BUF % 16 == 0, "16-byte stores");
+    static constexpr int PER = REC + 8 + 4;                      // bytes of a record's slot: record, source offset, score
+    static constexpr int ROUND = HD == 128 ? 256 : 128;
+    static constexpr int ROUND_MAX = 200 * 1024 / PER & ~7;      // one buffer that fills the SM
 };
 
 __device__ __forceinline__ void copy8_async(void* dst, const void* src) {
@@ -258,8 +266,8 @@ __device__ __forceinline__ void copy4_async(void* dst, const void* src) {
 template <int HD>
 __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     using C = MoveCfg<HD>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ long long s_off[2][C::ROUND];         // byte offset of the source record
+    extern __shared__ __align__(16) uint8_t smem[];              // per buffer: records, source offsets, scores
+    const int round = P.round, buf_bytes = round * C::PER;       // (a multiple of 8 records: 16-byte aligned parts)
     const int nb = P.cluster, rank = (int)blockIdx.x % nb;
     const int i = blockIdx.x / nb, kvh = blockIdx.y, tid = threadIdx.x;
     const bool isv = blockIdx.z != 0;
@@ -273,23 +281,24 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     uint8_t* cache = isv ? P.kvv : P.kvk;
     const float* sc_src = P.score + ((size_t)src * P.Hkv + kvh) * P.pstride;
     float* sc_dst = P.score + ((size_t)dst * P.Hkv + kvh) * P.pstride;
-    const int rounds = (stay + nb * C::ROUND - 1) / (nb * C::ROUND);
+    const int rounds = (stay + nb * round - 1) / (nb * round);
     // loads of a round into its buffer; false where every record of this CTA's part is where it belongs already
     auto load = [&](int rd) {
-        const int first = (rd * nb + rank) * C::ROUND, cnt = max(0, min(C::ROUND, stay - first));
-        uint8_t* buf = smem + (rd & 1) * C::BUF;
+        const int first = (rd * nb + rank) * round, cnt = max(0, min(round, stay - first));
+        uint8_t* buf = smem + (rd & 1) * buf_bytes;
+        long long* off = reinterpret_cast<long long*>(buf + round * C::REC);
         bool moves = false;
         for (int r = tid; r < cnt; r += MOVE_THREADS) {
             const int from = kept[first + r];
             moves |= from != first + r || src != dst;
-            s_off[rd & 1][r] = (long long)(kv_rec_index(P.pg, src, kvh, P.Hkv, P.pstride, from, P.status) * (size_t)C::REC);
-            if (!isv) copy4_async(buf + C::ROUND * C::REC + 4 * r, sc_src + from);
+            off[r] = (long long)(kv_rec_index(P.pg, src, kvh, P.Hkv, P.pstride, from, P.status) * (size_t)C::REC);
+            if (!isv) copy4_async(buf + round * (C::REC + 8) + 4 * r, sc_src + from);
         }
         moves = __syncthreads_or(moves);
         if (moves)
             for (int w = tid; w < cnt * C::WORDS; w += MOVE_THREADS) {
                 const int r = w / C::WORDS, c = w - r * C::WORDS;
-                copy8_async(buf + 8 * w, cache + s_off[rd & 1][r] + 8 * c);
+                copy8_async(buf + 8 * w, cache + off[r] + 8 * c);
             }
         asm volatile("cp.async.commit_group;" ::: "memory");
         return moves;
@@ -302,8 +311,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (nb > 1) cluster_sync(); else __syncthreads();        // every source of round rd has been read
         if (moves) {
-            const int first = (rd * nb + rank) * C::ROUND, cnt = min(C::ROUND, stay - first);
-            const uint8_t* buf = smem + (rd & 1) * C::BUF;
+            const int first = (rd * nb + rank) * round, cnt = min(round, stay - first);
+            const uint8_t* buf = smem + (rd & 1) * buf_bytes;
             for (int w = tid; w < cnt * C::REC / 16; w += MOVE_THREADS) {
                 // (an odd last record leaves a half piece, stored below; a piece never spans two pages)
                 const int r = 16 * w / C::REC;
@@ -319,7 +328,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
             }
             if (!isv)
                 for (int r = tid; r < cnt; r += MOVE_THREADS)
-                    sc_dst[first + r] = reinterpret_cast<const float*>(buf + C::ROUND * C::REC)[r];
+                    sc_dst[first + r] = reinterpret_cast<const float*>(buf + round * (C::REC + 8))[r];
         }
         moves = next;
         __syncthreads();                             // the buffer is free again

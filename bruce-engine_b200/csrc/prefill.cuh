@@ -267,6 +267,21 @@ template <int N> __device__ __forceinline__ void regs_grow() { asm volatile("set
 template <int N> __device__ __forceinline__ void regs_shrink() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// A warp's 32 columns of its 32 rows of split records, one row after the other: straight from the registers every store
+// would touch 32 rows of 8 bytes (128 rows of 256 dims took about 9 us), through 33-float rows of shared memory it is one run.
+// `rec`: this lane's row, null if it has none.
+__device__ __forceinline__ void store_record_columns(float* rec, int col, const uint32_t (&o)[32], float* stage, int lane) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) stage[lane * 33 + i] = __uint_as_float(o[i]);
+    __syncwarp();
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        float* row = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(rec), r));
+        if (row) row[col + lane] = stage[r * 33 + lane];
+    }
+    __syncwarp();
+}
+
 template <int HD, int BN, int VAR = VAR_PLAIN>
 __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
     using C = Cfg<HD, BN>;
@@ -781,7 +796,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         for (int c = 0; c < HD / 64; ++c) {
             uint32_t o[32];
             tmem_ld32(tmem + lane_base + C::T_O + half * (HD / 2) + c * 32, o);
-            if (row_ok) {
+            if (VAR != VAR_PLAIN && P.recs) {        // (the K operand is free: every product has completed)
+                store_record_columns(row_ok ? rec : nullptr, half * (HD / 2) + c * 32, o,
+                                     reinterpret_cast<float*>(Ksm) + warp * 32 * 33, lane);
+            } else if (row_ok) {
                 if (rec) {
                     float2* dst = reinterpret_cast<float2*>(rec + half * (HD / 2) + c * 32);    // records are 8-byte aligned
 #pragma unroll

@@ -679,7 +679,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         for (int c = 0; c < HD / 64; ++c) {
             uint32_t o[32];
             tmem_ld32(tmem + lane_base + T_O + L::ocol(2 * grp + c), o);
-            if (row_ok) {
+            if (VAR != VAR_PLAIN && P.recs) {        // (the K operand is free: every product has completed)
+                store_record_columns(row_ok ? rec : nullptr, grp * (HD / 2) + c * 32, o,
+                                     reinterpret_cast<float*>(Ksm) + warp * 32 * 33, lane);
+            } else if (row_ok) {
                 if (rec) {
                     float2* dst = reinterpret_cast<float2*>(rec + grp * (HD / 2) + c * 32);     // records are 8-byte aligned
 #pragma unroll

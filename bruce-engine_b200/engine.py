@@ -265,10 +265,10 @@ class AttnEngine:
     # ---- sliding window with sinks ---------------------------------------------------------------------
     def _dev(self, name: str, t, dtype, n: int = 0):
         """The pointer of a device tensor the new calls read or write, after the checks a raw pointer cannot have."""
-        if t.dtype is not dtype or not t.is_contiguous() or t.device != self.device or t.numel() < n:
-            raise ValueError(f"{name}: need a contiguous {dtype} tensor of at least {n} elements on {self.device}, "
-                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        return t.data_ptr()
+        if t.dtype is dtype and t.get_device() == self.device.index and t.is_contiguous() and t.numel() >= n:
+            return t.data_ptr()
+        raise ValueError(f"{name}: need a contiguous {dtype} tensor of at least {n} elements on {self.device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
     def _seqs(self, pos, sel, act):
         """Pointers of the per-sequence arrays: positions, partitions (or table rows) and activity."""
