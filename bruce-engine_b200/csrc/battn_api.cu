@@ -107,6 +107,16 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     if ((e = allow_smem(ev::k_evict_select<1024>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_select<512>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::ROUND_MAX * ev::MoveCfg<HD>::PER)) != cudaSuccess) return e;
+    {
+        cudaLaunchConfig_t cfg = {};                            // how many of its clusters run at once at one CTA per SM
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ev::MAX_CLUSTER; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        cfg.gridDim = dim3(ev::MAX_CLUSTER); cfg.blockDim = dim3(ev::MOVE_THREADS);
+        cfg.dynamicSmemBytes = ev::MoveCfg<HD>::ROUND_MAX * ev::MoveCfg<HD>::PER;
+        if ((e = cudaOccupancyMaxActiveClusters(&h->evict_clusters, ev::k_evict_move<HD>, &cfg)) != cudaSuccess) return e;
+    }
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 2, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
@@ -1172,13 +1182,18 @@ static int evict_impl(battn_handle* h, uint8_t* kvk, uint8_t* kvv, float* score,
     const int round_max = g.HD == 128 ? ev::MoveCfg<128>::ROUND_MAX : ev::MoveCfg<256>::ROUND_MAX;
     const int slot_bytes = g.HD == 128 ? ev::MoveCfg<128>::PER : ev::MoveCfg<256>::PER;
     for (c = 1; c < ev::MAX_CLUSTER && c * round < budget; ) c *= 2;
-    if (n_seq * g.Hkv * 2 * c <= h->num_sms) round = std::min(std::max(round, ((budget + c - 1) / c + 7) & ~7), round_max);
-    const bool one = c * round >= budget;
-    if (!one && 2 * round > round_max) round = round_max / 2 & ~7;
+    P.bufs = c * round >= budget ? 1 : 2;
+    if (n_seq * g.Hkv * 2 * c <= h->num_sms) {
+        const int half = g.HD == 128 ? ev::MoveCfg<128>::ROUND_HALF : ev::MoveCfg<256>::ROUND_HALF;
+        const int most = n_seq * g.Hkv * 2 <= h->evict_clusters ? round_max : half, part = (budget + c - 1) / c;
+        const int rounds = (part + most - 1) / most;
+        round = std::max(round, ((part + rounds - 1) / rounds + 7) & ~7);
+        P.bufs = 1;
+    }
     P.round = round;
     P.cluster = attr[0].val.clusterDim.x = c;
-    cfg.gridDim = dim3(n_seq * c, g.Hkv, 2); cfg.blockDim = dim3(ev::MOVE_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(one ? 1 : 2) * round * slot_bytes;
+    cfg.gridDim = dim3(n_seq * c, g.Hkv, 2); cfg.blockDim = dim3(round > round_max / 3 ? ev::MOVE_THREADS : 256);
+    cfg.dynamicSmemBytes = (size_t)P.bufs * round * slot_bytes;
     e = g.HD == 128 ? cudaLaunchKernelEx(&cfg, ev::k_evict_move<128>, P) : cudaLaunchKernelEx(&cfg, ev::k_evict_move<256>, P);
     h->launches += 2;
     if (e == cudaSuccess) e = cudaGetLastError();

@@ -40,6 +40,7 @@ struct battn_handle {
     int vw_ctas_per_sm;      // resident CTAs per SM of the wide verify kernel
     int fd_ctas_per_sm[3];   // resident CTAs per SM of the flash-decode kernel, per NT in {1,2}
     int fd_smem[3];
+    int evict_clusters;      // clusters of the eviction's move that are resident at one CTA per SM
     // Early KV streaming of the decode kernels (see fd::Params::early): allowed for a call when the last launch on
     // this handle wrote no cache rows other than the call's own (kvw_kind 0: none, 1: rows_per_seq rows at kvw_pos of
     // n_seq sequences, 2: anything else, 3: the appending decode call wrote one row per sequence into kvw_cache -- its

@@ -15,11 +15,12 @@ namespace battn {
 namespace ev {
 
 constexpr int MAX_CLUSTER = 8;              // the portable limit
-constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 512;           // 256 where several CTAs share an SM
 constexpr int KEYS_SMEM = 40 * 1024;        // keys a CTA keeps in shared memory at most (160 KB); a longer share re-reads the rest
 // Candidates that are worth another CTA of the cluster: up to here a pass over them is shorter than the cluster barriers
 // (4160 positions, one CTA of eight: 23 -> 12 us)
 constexpr int KEYS_PER_CTA = 8192;
+constexpr int MATCHES = 2048;               // keys of the first pass's bin that are listed
 
 struct Params {
     uint8_t* kvk;
@@ -36,7 +37,7 @@ struct Params {
     int Hkv, pstride, n_slots;
     int cluster;         // CTAs per cluster of this launch
     int keys;            // k_evict_select: keys its shared memory holds
-    int round;           // k_evict_move: records of a CTA in a round
+    int round, bufs;     // k_evict_move: records of a CTA in a round, buffers of that many
     int* status;
     Paging pg;
 };
@@ -135,14 +136,14 @@ __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_
 // CTAs share one (32 sequences of up to 8192: 20 -> 13 us)
 template <int SEL_THREADS>
 __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_select(const Params P) {
-    extern __shared__ uint32_t s_key[];              // P.keys keys of this CTA's share
+    extern __shared__ __align__(16) uint32_t s_key[];            // P.keys keys of this CTA's share
     __shared__ __align__(16) uint32_t s_hist[2048 + 2048 + 1024];
-    __shared__ uint32_t s_warp[32], s_found[3][2], s_low[2];
+    __shared__ uint32_t s_warp[32], s_found[3][2], s_low[2], s_match, s_list[MATCHES];
     __shared__ int s_clash;
     const int CL = P.cluster, rank = (int)blockIdx.x % CL;
     const int i = blockIdx.x / CL, kvh = blockIdx.y, tid = threadIdx.x;
     for (int b = tid; b < 2048 + 2048 + 1024; b += SEL_THREADS) s_hist[b] = 0;
-    if (tid == 0) { s_clash = 0; s_low[0] = s_low[1] = 0; }
+    if (tid == 0) { s_clash = 0; s_match = 0; s_low[0] = s_low[1] = 0; }
     pdl_wait();
     pdl_trigger();
     __syncthreads();
@@ -201,13 +202,24 @@ __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_selec
     // ---- the m-th best key ------------------------------------------------------------------------------------------------
     uint32_t T = 0, need = (uint32_t)m, gt_low = 0, eq_low = 0;
     descend<SEL_THREADS, 21, 11>(s_hist, C, rank, s_warp, s_found[0], T, need, gt_low, eq_low);
-    for (int j = tid; j < len; j += SEL_THREADS) {
-        const uint32_t k = key(j);
-        if ((k >> 21) == T) atomicAdd(&s_hist[2048 + ((k >> 10) & 2047)], 1u);
+    // one more look at every key; the third pass only needs those that matched, as long as their list has room
+    for (int j0 = 4 * tid; j0 < len; j0 += 4 * SEL_THREADS) {
+        uint4 k4;
+        if (j0 + 4 <= held) k4 = *reinterpret_cast<const uint4*>(s_key + j0);
+        else k4 = make_uint4(key(j0), j0 + 1 < len ? key(j0 + 1) : 0u, j0 + 2 < len ? key(j0 + 2) : 0u, j0 + 3 < len ? key(j0 + 3) : 0u);
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if ((k[e] >> 21) == T && j0 + e < len) {
+                atomicAdd(&s_hist[2048 + ((k[e] >> 10) & 2047)], 1u);
+                const uint32_t at = atomicAdd(&s_match, 1u);
+                if (at < MATCHES) s_list[at] = k[e];
+            }
     }
     descend<SEL_THREADS, 10, 11>(s_hist + 2048, C, rank, s_warp, s_found[1], T, need, gt_low, eq_low);
-    for (int j = tid; j < len; j += SEL_THREADS) {
-        const uint32_t k = key(j);
+    const bool listed = s_match <= MATCHES;
+    for (int j = tid; j < (listed ? (int)s_match : len); j += SEL_THREADS) {
+        const uint32_t k = listed ? s_list[j] : key(j);
         if ((k >> 10) == T) atomicAdd(&s_hist[4096 + (k & 1023)], 1u);
     }
     descend<SEL_THREADS, 0, 10>(s_hist + 4096, C, rank, s_warp, s_found[2], T, need, gt_low, eq_low);
@@ -225,9 +237,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_selec
     for (int base = 0; base < len; base += 4 * SEL_THREADS) {
         const int j0 = base + 4 * tid;
         uint32_t k[4], mine = 0;                     // two counts of 16 bits: better, equal
+        if (j0 + 4 <= held) {
+            const uint4 k4 = *reinterpret_cast<const uint4*>(s_key + j0);
+            k[0] = k4.x; k[1] = k4.y; k[2] = k4.z; k[3] = k4.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = j0 + e < len ? key(j0 + e) : 0u;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            k[e] = j0 + e < len ? key(j0 + e) : 0u;
             if (j0 + e < len) mine += (k[e] > T ? 0x10000u : 0u) + (k[e] == T ? 1u : 0u);
         }
         uint32_t tot;
@@ -246,13 +264,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_selec
 
 // A round of a CTA: P.round records, chosen by the host: all of the CTA's part in one round when there are few clusters (the
 // SM has the room, and a round costs two trips to memory one after the other: 4096 records of 272 bytes, 15 -> 9 us),
-// otherwise 34 KB, so that several CTAs share an SM.  Two buffers when there is more than one round.
+// half of it where the clusters would not all be resident at one CTA per SM (about nine of eight CTAs are: 16 clusters of 151 KB
+// ran in two waves, 22 us instead of 14), otherwise 34 KB, so that several CTAs share an SM and two buffers overlap the rounds.
 template <int HD>
 struct MoveCfg {
     static constexpr int REC = HD + HD / 16, WORDS = REC / 8;
     static constexpr int PER = REC + 8 + 4;                      // bytes of a record's slot: record, source offset, score
     static constexpr int ROUND = HD == 128 ? 256 : 128;
-    static constexpr int ROUND_MAX = 200 * 1024 / PER & ~7;      // one buffer that fills the SM
+    static constexpr int ROUND_MAX = 200 * 1024 / PER & ~7;      // one buffer that fills the SM, or half of it
+    static constexpr int ROUND_HALF = 108 * 1024 / PER & ~7;
 };
 
 __device__ __forceinline__ void copy8_async(void* dst, const void* src) {
@@ -267,9 +287,9 @@ template <int HD>
 __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     using C = MoveCfg<HD>;
     extern __shared__ __align__(16) uint8_t smem[];              // per buffer: records, source offsets, scores
-    const int round = P.round, buf_bytes = round * C::PER;       // (a multiple of 8 records: 16-byte aligned parts)
+    const int round = P.round, buf_bytes = P.bufs == 2 ? round * C::PER : 0;    // (a multiple of 8 records: 16-byte aligned parts)
     const int nb = P.cluster, rank = (int)blockIdx.x % nb;
-    const int i = blockIdx.x / nb, kvh = blockIdx.y, tid = threadIdx.x;
+    const int i = blockIdx.x / nb, kvh = blockIdx.y, tid = threadIdx.x, nt = blockDim.x;
     const bool isv = blockIdx.z != 0;
     pdl_wait();
     pdl_trigger();
@@ -288,15 +308,28 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
         uint8_t* buf = smem + (rd & 1) * buf_bytes;
         long long* off = reinterpret_cast<long long*>(buf + round * C::REC);
         bool moves = false;
-        for (int r = tid; r < cnt; r += MOVE_THREADS) {
-            const int from = kept[first + r];
-            moves |= from != first + r || src != dst;
-            off[r] = (long long)(kv_rec_index(P.pg, src, kvh, P.Hkv, P.pstride, from, P.status) * (size_t)C::REC);
-            if (!isv) copy4_async(buf + round * (C::REC + 8) + 4 * r, sc_src + from);
+        constexpr int UN = 4;
+        for (int r0 = tid; r0 < cnt; r0 += UN * nt) {            // the list and then the table are trips to memory: UN at once
+            int from[UN], page[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) from[u] = r0 + u * nt < cnt ? __ldg(kept + first + r0 + u * nt) : 0;
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                page[u] = P.pg.table ? __ldg(P.pg.table + (size_t)src * P.pg.max_pages + (from[u] >> P.pg.shift)) : 0;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int r = r0 + u * nt;
+                if (r >= cnt) break;
+                moves |= from[u] != first + r || src != dst;
+                off[r] = (long long)((P.pg.table ? kv_rec_index_page(P.pg, page[u], kvh, P.Hkv, from[u], P.status)
+                                                 : ((size_t)src * P.Hkv + kvh) * P.pstride + from[u]) * (size_t)C::REC);
+                if (!isv) copy4_async(buf + round * (C::REC + 8) + 4 * r, sc_src + from[u]);
+            }
         }
         moves = __syncthreads_or(moves);
         if (moves)
-            for (int w = tid; w < cnt * C::WORDS; w += MOVE_THREADS) {
+#pragma unroll 4
+            for (int w = tid; w < cnt * C::WORDS; w += nt) {
                 const int r = w / C::WORDS, c = w - r * C::WORDS;
                 copy8_async(buf + 8 * w, cache + off[r] + 8 * c);
             }
@@ -306,14 +339,19 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     bool moves = load(0);
     for (int rd = 0; rd < rounds; ++rd) {
         bool next = false;
-        if (rd + 1 < rounds) next = load(rd + 1);    // what is stored below lies under every source of this round
-        else asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (P.bufs == 2) {
+            if (rd + 1 < rounds) next = load(rd + 1);            // what is stored below lies under every source of this round
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
         if (nb > 1) cluster_sync(); else __syncthreads();        // every source of round rd has been read
         if (moves) {
             const int first = (rd * nb + rank) * round, cnt = min(round, stay - first);
             const uint8_t* buf = smem + (rd & 1) * buf_bytes;
-            for (int w = tid; w < cnt * C::REC / 16; w += MOVE_THREADS) {
+#pragma unroll 4
+            for (int w = tid; w < cnt * C::REC / 16; w += nt) {
                 // (an odd last record leaves a half piece, stored below; a piece never spans two pages)
                 const int r = 16 * w / C::REC;
                 uint8_t* to = cache + kv_rec_index(P.pg, dst, kvh, P.Hkv, P.pstride, first + r, P.status) * (size_t)C::REC +
@@ -327,11 +365,12 @@ __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
                 *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(buf + at);
             }
             if (!isv)
-                for (int r = tid; r < cnt; r += MOVE_THREADS)
+                for (int r = tid; r < cnt; r += nt)
                     sc_dst[first + r] = reinterpret_cast<const float*>(buf + round * (C::REC + 8))[r];
         }
-        moves = next;
         __syncthreads();                             // the buffer is free again
+        if (P.bufs == 1 && rd + 1 < rounds) next = load(rd + 1);
+        moves = next;
     }
 }
 
