@@ -163,7 +163,8 @@ inline int prefill_splits(const battn_handle* h, int rows, int is_swa, int var =
     int s = h->num_sms / ctas;
     // a share should keep at least 16 key tiles of 64, or the merge costs more than the split saves; a
     // sliding-window layer never has more than window/64 + 1 tiles per M tile
-    const int share = var == VAR_SINK ? 6 : 16, most = var == VAR_TRACK ? 32 : 8;
+    // (window with sinks: 201 rows in the 16/4/256 geometry with shares of 16, 6 and 4 tiles: 58, 46 and 31 us)
+    const int share = var == VAR_SINK ? 4 : 16, most = var == VAR_TRACK ? 32 : 8;
     if (is_swa && s > g.W / (64 * share)) s = g.W / (64 * share);
     return s < 1 ? 1 : (s > most ? most : s);
 }
@@ -499,10 +500,17 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
             M.n_slots = P.n_slots;
             M.stats = cv->stats; M.lse = cv->lse;
         }
+        if (cv) {
+            // several warps per item while the items alone do not fill the SMs
+            const int parts = rows * g.Hq <= h->num_sms * 16 ? g.HD / 64 : 1, warps = rows * g.Hq * parts;
+            const dim3 grid((warps + MERGE_M_THREADS / 32 - 1) / (MERGE_M_THREADS / 32)), block(MERGE_M_THREADS);
+            if (g.HD == 128) launch_pdl(parts > 1 ? k_merge_chunk<128, 2> : k_merge_chunk<128, 1>, grid, block, 0, st, M);
+            else             launch_pdl(parts > 1 ? k_merge_chunk<256, 4> : k_merge_chunk<256, 1>, grid, block, 0, st, M);
+        }
         // (head_dim 128: programmatic launch, the merge's blocks are resident and past their launch when the prompt
         // kernel drains -- 2 us less on a short chunk; at head_dim 256, where every 512-row chunk is split and the merge
         // has thousands of blocks, the early launch cost 2 % and the plain launch stays)
-        if (g.HD == 128) launch_pdl(k_merge<128>, dim3(rows * g.Hq), dim3(MERGE_THREADS), 0, st, M);
+        else if (g.HD == 128) launch_pdl(k_merge<128>, dim3(rows * g.Hq), dim3(MERGE_THREADS), 0, st, M);
         else             k_merge<256><<<rows * g.Hq, MERGE_THREADS, 0, st>>>(M);
         h->launches += 1;
         e = cudaGetLastError();

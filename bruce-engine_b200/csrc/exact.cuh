@@ -204,7 +204,7 @@ struct MergeParams {
     int count;             // REGULAR: splits; GATHERED: parts
     int log2_domain;       // records carry m in log2 units (flash-decode partials)
     int out_f16;
-    // REGULAR, and GATHERED behind a prompt chunk that may be idle (else null): skip rows of inactive sequences
+    // REGULAR and k_merge_chunk: skip rows of inactive sequences
     const int* pos; const int* kslot; const int* act;
     int is_swa, W, slot_ctx, n_slots;
     int* status;
@@ -214,7 +214,7 @@ struct MergeParams {
     // positions before the wait (pre_grid CTAs, pre_tile keys per tile) instead of read from the header after it
     int pre_grid, pre_tile;
     int cph;               // the decode kernel's cut: > 0: one sequence, cph CTAs per kv head; 0: linear
-    // GATHERED behind a weight-accumulating prompt chunk: its splits' statistics [split][row][head] = (m, l) in log2 units,
+    // k_merge_chunk behind a weight-accumulating prompt chunk: its splits' statistics [split][row][head] = (m, l) in log2 units,
     // joined into lse [row][head] = m + log2(l)
     const float2* stats;
     float* lse;
@@ -250,27 +250,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_merge(const MergeParams P) {
         base = P.part + (((size_t)rowidx * P.Hkv + kvh) * count * P.G + h) * (size_t)(HD + 2);
         stride = (size_t)P.G * (HD + 2);
     } else {                                     // MERGE_GATHERED
-        if (P.pos) {                             // the records of one prompt chunk, absent when its sequence was skipped
-            const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.n_rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
-            if (!sr.active) return;
-        }
         count = P.count;
         base = P.part + ((size_t)rowidx * P.Hq + hq) * (size_t)(HD + 2);
         stride = (size_t)P.n_rows * P.Hq * (HD + 2);
     }
     count = min(count, MERGE_MAX_COUNT);
 
-    if (P.stats && warp == 0) {
-        const size_t si = (size_t)rowidx * P.Hq + hq, step = (size_t)P.n_rows * P.Hq;
-        float2 st = lane < count ? P.stats[si + lane * step] : make_float2(NEG_BIG, 0.f);       // at most 32 splits
-        float M = st.x;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float L = st.y * fast_exp2(st.x - M);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (lane == 0) P.lse[si] = M + log2f(L);
-    }
     // phase 1: (m, l) of every record, block max of m
     float mx = NEG_BIG;
     for (int s = tid; s < count; s += MERGE_THREADS) {
@@ -595,6 +580,58 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_many(const MergeParam
     pdl_wait();
     const int item = blockIdx.x * (MERGE_M_THREADS / 32) + (threadIdx.x >> 5);
     if (item < P.n_rows * P.Hq) merge_many<HD>(P, item);
+}
+
+// The split records [split][row][head][HD + 2] of a prompt chunk's variants (see ChunkVariant), at most 32 splits: a warp per
+// (row, head) as above, lane s with split s, and the log-sum-exps of a weight-accumulating chunk.  (201 rows x 16 heads of
+// four records: 7 us, where k_merge's blocks took 12.)  PARTS > 1: that many warps per item share its dims, with more loads in
+// flight, for short chunks with many splits (32 rows x 16 heads of 32 records: 21 us by one warp, 14 by four).
+template <int HD, int PARTS>
+__global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_chunk(const MergeParams P) {
+    constexpr int Q2 = HD / 64 / PARTS;                          // float2s per lane (records are 8-byte aligned)
+    constexpr int UN = 16 / Q2;
+    pdl_trigger();
+    pdl_wait();
+    const SeqRange sr = seq_range(P.pos, P.kslot, P.act, 0, P.n_rows, P.is_swa, P.W, P.slot_ctx, P.n_slots, P.status);
+    const int warp = blockIdx.x * (MERGE_M_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int item = warp / PARTS, d0 = warp % PARTS * (HD / PARTS);
+    const size_t items = (size_t)P.n_rows * P.Hq;
+    if (!sr.active || item >= (int)items) return;
+    const float* base = P.part + (size_t)item * (HD + 2);
+    const size_t stride = items * (HD + 2);
+    const float2 ml = lane < P.count ? *reinterpret_cast<const float2*>(base + lane * stride + HD) : make_float2(NEG_BIG, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    const float w = fast_exp2(ml.x - M);
+    float L = w * ml.y;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+    if (P.stats) {                                               // the records' m, with denominators of unrounded weights
+        float Lx = lane < P.count ? P.stats[item + lane * items].y * w : 0.f;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) Lx += __shfl_xor_sync(0xffffffffu, Lx, d);
+        if (lane == 0 && d0 == 0) P.lse[item] = M + log2f(Lx);
+    }
+    float2 acc[Q2];
+#pragma unroll
+    for (int j = 0; j < Q2; ++j) acc[j] = make_float2(0.f, 0.f);
+#pragma unroll UN
+    for (int s = 0; s < P.count; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+        for (int j = 0; j < Q2; ++j) {
+            const float2 o = *reinterpret_cast<const float2*>(base + s * stride + d0 + 2 * (lane + 32 * j));
+            acc[j].x = fmaf(o.x, ws, acc[j].x); acc[j].y = fmaf(o.y, ws, acc[j].y);
+        }
+    }
+    const float il = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int j = 0; j < Q2; ++j) {
+        const size_t oi = (size_t)item * HD + d0 + 2 * (lane + 32 * j);
+        if (P.out_f16) reinterpret_cast<__half2*>(P.out)[oi >> 1] = __floats2half2_rn(acc[j].x * il, acc[j].y * il);
+        else *reinterpret_cast<float2*>(reinterpret_cast<float*>(P.out) + oi) = make_float2(acc[j].x * il, acc[j].y * il);
+    }
 }
 
 // The receiving half of the exchange on its own: one block per (row, head) waits for every device's record of the
