@@ -157,7 +157,15 @@ __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_selec
         const int sj = P.kslot ? P.kslot[j] : 0, dj = P.kslot_dst ? P.kslot_dst[j] : sj;
         if (dj == dst || sj == dst) s_clash = 1;
     }
-    if (P.n_seq > 1) __syncthreads();
+    // ... and so would page 0 be in the place of a page that is not mapped
+    if (P.pg.table && !bad) {
+        const int from = (n + (1 << P.pg.shift) - 1) >> P.pg.shift, to = (min(n, P.budget) + (1 << P.pg.shift) - 1) >> P.pg.shift;
+        for (int j = tid; j < from + to; j += SEL_THREADS) {
+            const int e = P.pg.table[(size_t)(j < from ? src : dst) * P.pg.max_pages + (j < from ? j : j - from)];
+            if ((unsigned)e >= (unsigned)P.pg.n_pages) s_clash = 1;
+        }
+    }
+    __syncthreads();
     bad = bad || s_clash;
     const int stay = min(n, P.budget);
     if (kvh == 0 && rank == 0 && tid == 0) {

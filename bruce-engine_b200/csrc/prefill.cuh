@@ -312,7 +312,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         return;
     }
     const int kv_slot = chunk_slot<VAR>(P, tid == 0);
-    if (VAR != VAR_PLAIN && kv_slot < 0) return;
+    if (VAR != VAR_PLAIN && kv_slot < 0) {                   // (both CTAs of a pair alike)
+        if (early) pdl_wait();                               // a grid that ends before its predecessor breaks the chain of waits
+        return;
+    }
     const int rbase = mt * MR;
     const int rows_eff = min(MR, P.rows - rbase);
     const int p_first = p0 + rbase, p_last = p_first + rows_eff - 1;

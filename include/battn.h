@@ -419,9 +419,10 @@ int battn_attend_track_paged(battn_handle* h, void* out, float* score_out, const
  *   kslot_dst  NULL: in place.  Otherwise the partition (or table row) that receives sequence i, which another sequence of
  *              the call must neither read nor write (a clash sets BATTN_DEV_BAD_POSITION and skips it); the source
  *              keeps its records and scores.  So a conversation can be trimmed out of a prompt that others share.
- *   paged      the pages behind the first min(n, budget) positions of the target row must be mapped, and in place not
- *              shared with another sequence (un-share them first, as before an append); pages past them are free
- *              afterwards.  Two rows of one call may share source pages; a target page is in no other place of the call.
+ *   paged      the pages behind the first n positions of the source row and the first min(n, budget) of the target row must
+ *              be mapped (a table entry outside the pool sets BATTN_DEV_BAD_POSITION and skips the sequence), and the target's
+ *              in place not shared with another sequence (un-share them first, as before an append); pages past them are
+ *              free afterwards.  Two rows of one call may share source pages; a target page is in no other place of the call.
  *   ws         battn_evict_workspace_bytes(n_seq)
  * Sequences with act[i] == 0 or a bad position or slot are left alone, their kept and pos_out too.  The result does not
  * depend on timing: no floating-point sum is formed, and records are copied. */

@@ -199,6 +199,32 @@ def test_bad_positions_slots_and_clashes_set_the_status_bit():
     assert run([100, 100], [0, 0], [2, 3])[:2] == (0, [32, 32])
 
 
+def test_an_unmapped_page_skips_the_sequence():
+    """A hole among the source's or the target's pages sets the status bit; the sequence, and page 0, stay as they are."""
+    from bruce_engine_b200 import capi
+    g = R.geom("B", slot_ctx=512, n_slots=1)
+    e = R.engine(g)
+    part = e.alloc_evict_part(2)
+    for hole, ok in (((0, 1), False), ((0, 2), True), ((2, 0), False), ((2, 1), True), (None, True)):
+        table = np.arange(16, dtype=np.int32).reshape(4, 4)
+        if hole:
+            table[hole] = (-1, 16)[hole[1] & 1]
+        tab = torch.from_numpy(table).to(e.device)
+        pool = [torch.randint(0, 256, (16 * g.n_kv * 128 * g.rec,), dtype=torch.uint8, device=e.device) for _ in range(2)]
+        before = [x.clone() for x in pool]
+        desc = capi.CPages(pool[0].data_ptr(), pool[1].data_ptr(), tab.data_ptr(), 16, 4, 4, 128)
+        score = torch.rand(4, g.n_kv, 512, device=e.device)
+        kept = torch.full((2, g.n_kv, 100), -9, dtype=torch.int32, device=e.device)
+        out = R.ids([-9, -9], e)
+        # sequence 0 holds pages 0 and 1 of its row and fills one page of row 2; sequence 1 is sound
+        e.evict_paged(desc, score, kept, out, R.ids([200, 130], e), part, 100, ktab=R.ids([0, 1], e), ktab_dst=R.ids([2, 3], e))
+        torch.cuda.synchronize()
+        assert e.device_status() == (0 if ok else 1) and out.tolist() == [100 if ok else -9, 100], hole
+        for a, b in zip(pool, before):
+            a, b = a.reshape(16, -1), b.reshape(16, -1)
+            assert torch.equal(a[:8], b[:8]) and torch.equal(a[8], b[8]) == (not ok) and not torch.equal(a[12], b[12])
+
+
 def test_refusals():
     from bruce_engine_b200 import capi
     g = R.geom("B", slot_ctx=256, n_slots=2)

@@ -206,6 +206,22 @@ def test_bad_positions_and_slots_set_the_status_bit():
             assert e.device_status() == 1 and torch.isnan(out).all(), (rows, p, s)
 
 
+def test_an_unmapped_page_that_is_needed_sets_the_status_bit():
+    """Pages between the sinks and the window may be missing, those the rows see may not (page 0 is read in their place)."""
+    g = R.geom("B", window=128, slot_ctx=1024)
+    e = R.engine(g)
+    q, k, v = R.draw(g, 900, 100, 3)
+    recs = [R.quantised(g, k, v)]
+    for rows in (1, 8, 100):
+        for page, status in ((3, 0), (0, 1), (6, 1)):
+            pg = R.Paged(e, recs, 0, 128, 5, skip=lambda i, p: p == page)
+            out = new_out(e, 1, rows, g.n_head, g.head_dim)
+            e.attn_sinks_paged(out, dev_q(e, q[None, :rows]), pg.desc, e.sinks(4), R.ids([900 - rows], e), e.alloc_part(1, rows),
+                               rows=rows)
+            torch.cuda.synchronize()
+            assert e.device_status() == status, (rows, page)
+
+
 def test_refusals():
     from bruce_engine_b200 import capi
     g = R.geom("B", window=128, slot_ctx=512, n_slots=2)
