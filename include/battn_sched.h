@@ -137,7 +137,9 @@ public:
      * shared.  Returns the number of positions dst now holds (a multiple of the page length). */
     int share_prefix(int src, int dst, int n_pos) {
         if (used_[(size_t)dst] != 0) return 0;
-        const int n = std::min(n_pos / page_len_, used_[(size_t)src]);
+        int n = std::min(n_pos / page_len_, used_[(size_t)src]);
+        for (int i = 0; i < n; ++i)
+            if (at(src, i) < 0) n = i;                                   /* a dropped page ends what can be shared */
         for (int i = 0; i < n; ++i) {
             at(dst, i) = at(src, i);
             ++ref_[(size_t)at(src, i)];
@@ -152,6 +154,7 @@ public:
     bool make_writable(int row, int pos, int* from, int* to) {
         *from = *to = -1;
         int& p = at(row, pos / page_len_);
+        if (p < 0) return false;
         if (ref_[(size_t)p] <= 1) return true;
         if (free_.empty()) return false;
         const int q = free_.back();
@@ -166,12 +169,26 @@ public:
     /* Drops the row's pages; a page returns to the pool when its last row lets go of it. */
     void release(int row) {
         for (int i = 0; i < used_[(size_t)row]; ++i) {
-            int& p = at(row, i);
-            if (--ref_[(size_t)p] == 0) free_.push_back(p);
-            p = -1;
+            unmap(row, i);
         }
         used_[(size_t)row] = 0;
         dirty_[(size_t)row] = 1;
+    }
+    /* Bounded caches.  trim: the row holds n_pos positions from now on (behind battn_evict_paged: min(n, budget)); pages
+     * past them return to the pool.  drop: the pages that lie wholly inside [from, to) return to the pool and leave holes,
+     * for rows whose window has passed them (battn_attend_sinks_paged: from = n_sink, to = pos + 1 - window).  Call
+     * them once the launches that still read those pages are enqueued, and upload the row before the next ones. */
+    void trim(int row, int n_pos) {
+        const int keep = (n_pos + page_len_ - 1) / page_len_;
+        int& have = used_[(size_t)row];
+        if (keep >= have) return;
+        for (; have > keep; --have) unmap(row, have - 1);
+        dirty_[(size_t)row] = 1;
+    }
+    void drop(int row, int from, int to) {
+        const int a = (std::max(from, 0) + page_len_ - 1) / page_len_, b = std::min(to / page_len_, used_[(size_t)row]);
+        for (int i = a; i < b; ++i)
+            if (unmap(row, i)) dirty_[(size_t)row] = 1;
     }
     const int* table() const { return table_.data(); }                  /* [n_rows][max_pages], -1 = unmapped */
     const int* row(int r) const { return table_.data() + (size_t)r * max_pages_; }
@@ -183,6 +200,13 @@ public:
 
 private:
     int& at(int r, int i) { return table_[(size_t)r * max_pages_ + i]; }
+    bool unmap(int r, int i) {
+        int& p = at(r, i);
+        if (p < 0) return false;
+        if (--ref_[(size_t)p] == 0) free_.push_back(p);
+        p = -1;
+        return true;
+    }
     int page_len_, max_pages_;
     std::vector<int> table_, used_, ref_;
     std::vector<char> dirty_;

@@ -1,6 +1,9 @@
 """The bounded-cache calls without a device: argument checks that need no handle, and the plain eviction list against its
 definition."""
 import ctypes as C
+import os
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -44,3 +47,16 @@ def test_the_plain_list_is_the_definition(n, budget, n_sink, n_recent):
         left = [worth(i) for i in mid if i not in held]
         kept = [worth(i) for i in mid if i in held]
         assert not kept or not left or min(kept) > max(left)
+
+
+def test_pages_of_bounded_rows_return_to_the_pool(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "bounded_pages_test")
+    r = subprocess.run([gxx, "-std=c++17", "-O1", "-pthread", "-Wall", "-Wextra", "-I", os.path.join(root, "include"),
+                        os.path.join(root, "tests", "host", "bounded_pages_test.cpp"), "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.strip() == "OK", r.stdout + r.stderr
