@@ -422,7 +422,7 @@ struct ChunkVariant {
     const int* act;
     SinkView sink;               // VAR_SINK
     float2* stats;               // VAR_TRACK, see pf::Params
-    float* lse;
+    float2* norm;
 };
 
 // prompt chunk on the tcgen05 kernel: one CTA per (128-row M tile, kv head), normalised output
@@ -442,7 +442,7 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
     const int var = cv ? cv->var : VAR_PLAIN;
     if (cv) {
         P.kslot = cv->kslot; P.act = cv->act; P.n_slots = pv ? pv->n_tables : g.n_slots; P.sink = cv->sink;
-        P.stats = cv->stats; P.lse = cv->lse;
+        P.stats = cv->stats; P.norm = cv->norm;
     }
     // early KV streaming: only behind the append / prologue of exactly this chunk, or no cache write
     P.early = h->early_stream &&
@@ -498,7 +498,7 @@ int launch_prefill(battn_handle* h, void* out, const void* q, const uint8_t* kvk
         if (cv) {                                // an idle sequence left no records
             M.pos = pos; M.kslot = cv->kslot; M.act = cv->act; M.is_swa = is_swa; M.W = g.W; M.slot_ctx = P.slot_ctx;
             M.n_slots = P.n_slots;
-            M.stats = cv->stats; M.lse = cv->lse;
+            M.stats = cv->stats; M.norm = cv->norm;
         }
         if (cv) {
             // several warps per item while the items alone do not fill the SMs
@@ -1057,17 +1057,17 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
 }
 
 // ---- attention that accumulates its weights -----------------------------------------------------------------------
-// scratch of a prompt chunk: split records, their statistics, the rows' log-sum-exps
+// scratch of a prompt chunk: split records, their statistics, the rows' normalisers
 struct TrackChunkWs {
-    size_t stats, lse, total;
+    size_t stats, norm, total;
 };
 static TrackChunkWs track_chunk_workspace(const battn_handle* h, int rows) {
     const size_t per = (size_t)rows * h->g.Hq;
     TrackChunkWs w;
     const int splits = prefill_splits(h, rows, 0, VAR_TRACK);
     w.stats = align_up(exact_workspace(h, 1, rows, splits), 256);
-    w.lse = w.stats + align_up(per * splits * sizeof(float2), 256);
-    w.total = w.lse + align_up(per * sizeof(float), 256);
+    w.norm = w.stats + align_up(per * splits * sizeof(float2), 256);
+    w.total = w.norm + align_up(per * sizeof(float2), 256);
     return w;
 }
 
@@ -1109,10 +1109,10 @@ static int attend_track_impl(battn_handle* h, void* out, float* score_out, const
         const TrackChunkWs cw = track_chunk_workspace(h, rows);
         if (ws_bytes < cw.total) return BATTN_ERR_CAPACITY;
         if (g.W < 64) return BATTN_ERR_ARG;                     // as battn_prefill
-        ChunkVariant cv{VAR_TRACK, kslot, act, {}, reinterpret_cast<float2*>(w + cw.stats), reinterpret_cast<float*>(w + cw.lse)};
+        ChunkVariant cv{VAR_TRACK, kslot, act, {}, reinterpret_cast<float2*>(w + cw.stats), reinterpret_cast<float2*>(w + cw.norm)};
         if ((rc = launch_prefill(h, out, q, kvk, kvv, pos, ws, rows, 0, st, nullptr, pv, 0, &cv))) return rc;
         tr::ChunkParams P;
-        P.q = q; P.kvk = kvk; P.lse = cv.lse; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot; P.act = act;
+        P.q = q; P.kvk = kvk; P.norm = cv.norm; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot; P.act = act;
         P.rows = rows; P.Hq = g.Hq; P.Hkv = g.Hkv; P.G = g.G; P.q_f16 = g.q_f16;
         P.pstride = pv ? pv->capacity : g.slot_ctx; P.n_slots = pv ? pv->n_tables : g.n_slots;
         P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;

@@ -215,9 +215,9 @@ struct MergeParams {
     int pre_grid, pre_tile;
     int cph;               // the decode kernel's cut: > 0: one sequence, cph CTAs per kv head; 0: linear
     // k_merge_chunk behind a weight-accumulating prompt chunk: its splits' statistics [split][row][head] = (m, l) in log2 units,
-    // joined into lse [row][head] = m + log2(l)
+    // joined into norm [row][head] = (m, 1 / l)
     const float2* stats;
-    float* lse;
+    float2* norm;
     // sequence split across devices (k_merge_balanced as the pushing epilogue, k_merge_wait): see XchgView
     XchgView xchg;
 };
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_many(const MergeParam
 }
 
 // The split records [split][row][head][HD + 2] of a prompt chunk's variants (see ChunkVariant), at most 32 splits: a warp per
-// (row, head) as above, lane s with split s, and the log-sum-exps of a weight-accumulating chunk.  (201 rows x 16 heads of
+// (row, head) as above, lane s with split s, and the normalisers of a weight-accumulating chunk.  (201 rows x 16 heads of
 // four records: 7 us, where k_merge's blocks took 12.)  PARTS > 1: that many warps per item share its dims, with more loads in
 // flight, for short chunks with many splits (32 rows x 16 heads of 32 records: 21 us by one warp, 14 by four).
 template <int HD, int PARTS>
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_chunk(const MergePara
         float Lx = lane < P.count ? P.stats[item + lane * items].y * w : 0.f;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) Lx += __shfl_xor_sync(0xffffffffu, Lx, d);
-        if (lane == 0 && d0 == 0) P.lse[item] = M + log2f(Lx);
+        if (lane == 0 && d0 == 0) P.norm[item] = make_float2(M, 1.f / Lx);
     }
     float2 acc[Q2];
 #pragma unroll

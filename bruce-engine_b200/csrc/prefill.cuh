@@ -84,9 +84,10 @@ struct Params {
     SinkView sink;               // VAR_SINK
     // VAR_TRACK: the softmax statistics of every (row, head) in log2 units, with the denominator summed in fp32 from the
     // unrounded weights (the weights that are accumulated divide by it; the output divides by the sum of the rounded ones).
-    // One split: lse [row][head] = m + log2(l).  Several: stats [split][row][head] = (m, l), joined by the merge.
+    // One split: norm [row][head] = (m, 1 / l).  Several: stats [split][row][head] = (m, l), joined by the merge.  m and l stay
+    // apart: as m + log2(l), a sum near 16, they would be rounded by 2^-21, ten times what the weights are off otherwise.
     float2* stats = nullptr;
-    float* lse = nullptr;
+    float2* norm = nullptr;
 };
 // the partition (or table row) of a variant's sequence; -1: idle or bad, nothing to do
 template <int VAR>
@@ -784,7 +785,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
             const bool some = m_ref > 0.5f * NEG_BIG;
             if (row_ok && half == 0) {
                 if (P.recs) P.stats[si] = make_float2(some ? m_ref * c2 : NEG_BIG, le);
-                else P.lse[si] = m_ref * c2 + log2f(le);
+                else P.norm[si] = make_float2(m_ref * c2, 1.f / le);
             }
         }
         const float il = l > 0.f ? 1.f / l : 0.f;

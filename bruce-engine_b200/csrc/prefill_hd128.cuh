@@ -44,6 +44,9 @@
 // chosen so that every shared-memory access of the dequant warps is bank-conflict free.
 // Every wait is bounded; a wait that runs out sets the device status word, the remaining waits are
 // skipped, tensor memory is released and the kernel returns.
+// Variants (template parameter VAR, see common.cuh): VAR_SINK walks the sink tiles before the window's; VAR_TRACK also sums the
+// unrounded weights per row (two adds per two exponentials, not measurable beside the plain kernel) for the accumulation
+// in track.cuh.
 #pragma once
 #include "prefill.cuh"
 
@@ -665,7 +668,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             const bool some = m_ref > 0.5f * NEG_BIG;
             if (row_ok && grp == 0) {
                 if (P.recs) P.stats[si] = make_float2(some ? m_ref * c2 : NEG_BIG, le);
-                else P.lse[si] = m_ref * c2 + log2f(le);
+                else P.norm[si] = make_float2(m_ref * c2, 1.f / le);
             }
         }
         const float il = l > 0.f ? 1.f / l : 0.f;

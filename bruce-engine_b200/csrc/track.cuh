@@ -1,7 +1,7 @@
 // The weights of an attention call, accumulated per cached position: score_out[kv head][p] = score_in[kv head][p] + the sum
-// over the call's rows and the heads of the group of w = 2^(s - lse), where s is the row's score of key p in log2 units and
-// lse its log-sum-exp.  The attention kernels (VAR_TRACK) leave what is needed for lse, with denominators summed in fp32
-// from unrounded weights.
+// over the call's rows and the heads of the group of w = 2^(s - m) / l, where s is the row's score of key p in log2 units, m
+// the reference its attention used and l = sum 2^(s - m).  The attention kernels (VAR_TRACK) leave m and l, with l summed in
+// fp32 from unrounded weights.
 //
 // track_step, one row per sequence: the decode kernel kept the scores (16 bytes per position and kv head at four heads,
 // beside the 272 bytes of K and V it streams), so the cache is not read again; it runs beside the merge of the split records,
@@ -35,8 +35,8 @@ struct StepMerge {           // one launch: blocks below `merge_blocks` merge th
     int merge_blocks;
 };
 
-// log-sum-exp of head `h` of an item over the records of the CTAs that hold a piece of it, by one warp
-__device__ __forceinline__ float item_lse(const StepParams& P, int item, int clo, int chi, int h, int lane) {
+// (m, 1 / l) of head `h` of an item over the records of the CTAs that hold a piece of it, by one warp
+__device__ __forceinline__ float2 item_norm(const StepParams& P, int item, int clo, int chi, int h, int lane) {
     const float* rec = P.part + ((size_t)(clo + item) * P.G + h) * (P.HD + 4) + P.HD;
     const size_t step = (size_t)P.G * (P.HD + 4);
     float M = NEG_BIG, L = 0.f;
@@ -52,14 +52,14 @@ __device__ __forceinline__ float item_lse(const StepParams& P, int item, int clo
     L *= fast_exp2(M - Mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    return Mx + log2f(L);
+    return make_float2(Mx, 1.f / L);
 }
 
 // Block `cta` of `n_cta` accumulates its contiguous share of the scores' tiles, a thread per position, four in flight.
 template <int THREADS>
 __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_cta) {
     extern __shared__ int s_cum[];                               // [n_seq + 1]
-    __shared__ float s_lse[8];
+    __shared__ float2 s_norm[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i <= P.n_seq; i += THREADS) s_cum[i] = P.hdr[2 + i];
     const int per_cta = P.hdr[0];
@@ -73,10 +73,10 @@ __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_c
         const int p = P.pos[pc.i], slot = P.kslot ? P.kslot[pc.i] : 0;
         int clo, chi;
         fd::item_ctas(P.cph, per_cta, P.Hkv, c0, nt, pc.kvh, clo, chi);
-        __syncthreads();                                         // the previous piece has used s_lse
+        __syncthreads();                                         // the previous piece has used s_norm
         if (warp < P.G) {
-            const float lse = item_lse(P, pc.i * P.Hkv + pc.kvh, clo, chi, warp, lane);
-            if (lane == 0) s_lse[warp] = lse;
+            const float2 nm = item_norm(P, pc.i * P.Hkv + pc.kvh, clo, chi, warp, lane);
+            if (lane == 0) s_norm[warp] = nm;
         }
         __syncthreads();
         const int first = pc.tl * TILE, keys = min(pc.n * TILE, p + 1 - first);
@@ -85,7 +85,7 @@ __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_c
         const float* sc = P.scores + (size_t)g * TILE * P.G;
         constexpr int UN = 4;
         if (P.G == 4) {                                          // the usual group: a position's scores are one 16-byte load
-            const float l0 = s_lse[0], l1 = s_lse[1], l2 = s_lse[2], l3 = s_lse[3];
+            const float2 n0 = s_norm[0], n1 = s_norm[1], n2 = s_norm[2], n3 = s_norm[3];
             for (int k0 = tid; k0 < keys; k0 += UN * THREADS) {
                 float4 v[UN];
                 float w[UN];
@@ -99,13 +99,14 @@ __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_c
                 for (int u = 0; u < UN; ++u) {
                     const int k = k0 + u * THREADS;
                     if (k < keys)
-                        out[k] = ((fast_exp2(v[u].x - l0) + fast_exp2(v[u].y - l1)) + (fast_exp2(v[u].z - l2) + fast_exp2(v[u].w - l3))) + w[u];
+                        out[k] = (fmaf(fast_exp2(v[u].x - n0.x), n0.y, fast_exp2(v[u].y - n1.x) * n1.y) +
+                                  fmaf(fast_exp2(v[u].z - n2.x), n2.y, fast_exp2(v[u].w - n3.x) * n3.y)) + w[u];
                 }
             }
         } else {
             for (int k = tid; k < keys; k += THREADS) {
                 float w = 0.f;
-                for (int h = 0; h < P.G; ++h) w += fast_exp2(sc[(size_t)k * P.G + h] - s_lse[h]);
+                for (int h = 0; h < P.G; ++h) w = fmaf(fast_exp2(sc[(size_t)k * P.G + h] - s_norm[h].x), s_norm[h].y, w);
                 out[k] = w + (in && first + k < p ? in[k] : 0.f);
             }
         }
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_track_many(const Step
 struct ChunkParams {
     const void* q;
     const uint8_t* kvk;
-    const float* lse;        // [row][head]
+    const float2* norm;      // [row][head]: (m, 1 / l)
     float* out;
     const float* in;
     const int* pos;
@@ -160,10 +161,12 @@ struct ChunkParams {
 //     every product, and a 128-column product with both operands there runs into the shared-memory bandwidth.
 //   * Q tiles of 128 (row, head) pairs stream from L2 through a ring as the B operand; every one serves all keys of the unit
 //     (two M tiles at head_dim 128: half the L2 traffic, which at one would be near 7 TB/s).
-//   * Two accumulators of 128 columns; each of two groups of four warps empties its own: w += 2^(s c - lse), one exponential
+//   * Two accumulators of 128 columns; each of two groups of four warps empties its own: w += 2^(s c - m) / l, one exponential
 //     per score.  The exponentials (16 per cycle and SM) take as long as the two products: that balance is the bound.
 //   * Between units the eight warps convert the next K, whose raw records were fetched ahead.
-// Against the form with warp MMAs and scales applied to fp32 sums (512 rows at 32K, 8 kv heads): 705 -> 262 us.
+//   * The Q loader shifts instead of dividing (the group is a power of two): with divisions it was the bound.
+// 512 rows at 32K, 32/8 heads of 128: 245 us at 1.6 GHz (warp MMAs with scales on fp32 sums took 705, the divisions 390);
+// exponentials 62 % of their rate, tensor pipe 60 %.
 constexpr int QN = 128;                     // pairs per Q tile
 constexpr int CTHREADS = 14 * 32;           // warps 0-7 convert K and sum weights, 8-11 load Q, 12 issues the MMAs, 13 loads K
 constexpr int MAX_PAIRS = MAX_PREFILL * 8;
@@ -178,8 +181,8 @@ struct ChunkCfg {
     static constexpr int QST = HD == 128 ? 4 : 2;                // Q ring
     static constexpr int RAW = 128 * REC;                        // raw records of one key tile
     static constexpr int OFF_RAW = QST * Q_BYTES;
-    static constexpr int OFF_LSE = OFF_RAW + KT * RAW;           // -lse of every pair of the unit's kv head
-    static constexpr int OFF_XCH = OFF_LSE + MAX_PAIRS * 4;
+    static constexpr int OFF_NORM = OFF_RAW + KT * RAW;          // -m, then 1 / l, of every pair of the unit's kv head
+    static constexpr int OFF_XCH = OFF_NORM + MAX_PAIRS * 8;
     static constexpr int OFF_BAR = OFF_XCH + 128 * 4;
     static constexpr int SMEM = OFF_BAR + 16 * 8 + 16 + 1024;    // + slack to align the base to 1024
     static constexpr int T_LO = HD / 2;                          // columns from the high to the low part of a K tile
@@ -195,7 +198,8 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
     constexpr int NBLK = C::NBLK, REC = C::REC, KT = C::KT, QST = C::QST;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    float* s_nl = reinterpret_cast<float*>(smem + C::OFF_LSE);
+    float* s_nm = reinterpret_cast<float*>(smem + C::OFF_NORM);
+    float* s_il = s_nm + MAX_PAIRS;
     float* s_xch = reinterpret_cast<float*>(smem + C::OFF_XCH);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_BAR + 16 * 8);    // [0] tmem base, [1] abort
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
         uint32_t used = 0, steps = 0, unit = 0;                  // accumulators emptied by this group, products so far, units
         for (int u = blockIdx.x; u < units; u += gridDim.x, ++unit) {
             const int kvh = u % P.Hkv, t0 = unit_t0(u), qt0 = unit_qt0(t0);
-            // every product of the previous unit has completed (each group has seen its last one), s_nl and s_xch are read
+            // every product of the previous unit has completed (each group has seen its last one), s_nm, s_il and s_xch are read
             named_bar_sync(1, 256);
             wait(B_RAWF, unit & 1);
             if (KT == 1 || grp < unit_tiles(t0)) {
@@ -277,15 +281,17 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
             tc_fence_before();
             __syncwarp();
             if (lane == 0) { mbar_arrive(&bars[B_RAWE]); mbar_arrive(&bars[B_KRDY]); }
-            // -lse of every pair, while the first products run
-            for (int i = tid + qt0 * QN; i < n_qt * QN; i += 256)
-                s_nl[i] = i < pairs ? -P.lse[(size_t)(i >> lg) * P.Hq + kvh * G + (i & (G - 1))] : NEG_BIG;    // no pair: weight 0
+            // the pairs' normalisers, while the first products run (no pair: weight 0)
+            for (int i = tid + qt0 * QN; i < n_qt * QN; i += 256) {
+                const float2 nm = i < pairs ? P.norm[(size_t)(i >> lg) * P.Hq + kvh * G + (i & (G - 1))] : make_float2(0.f, 0.f);
+                s_nm[i] = -nm.x; s_il[i] = nm.y;
+            }
             named_bar_sync(1, 256);
             const int key = t0 + (KT == 2 ? 128 * grp : 0) + row;
             const bool mine = KT == 1 || grp < unit_tiles(t0);
             const uint32_t tD = tmem + lane_base + C::T_D + grp * 128;
             const uint64_t c2p = pack_f2(P.scale_log2, P.scale_log2);
-            float w0 = 0.f, w1 = 0.f;
+            float w = 0.f;
             for (int qt = qt0; qt < n_qt; ++qt, ++steps) {
                 if (KT == 2 ? !mine : (int)(steps & 1) != grp) continue;
                 wait(B_DF + grp, used & 1);
@@ -305,31 +311,36 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&bars[B_DE + grp]);
                     }
-                    const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(s_nl + qt * QN + 64 * h);
+                    const ulonglong2* nm = reinterpret_cast<const ulonglong2*>(s_nm + qt * QN + 64 * h);
+                    const float4* il = reinterpret_cast<const float4*>(s_il + qt * QN + 64 * h);
+                    float a[4] = {0.f, 0.f, 0.f, 0.f};           // sums of 16 terms each: what a long sum would round away
                     if (!masked) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const ulonglong2 l = nl[i];
+                            const ulonglong2 l = nm[i];
+                            const float4 r = il[i];
                             float e0, e1, e2, e3;
                             ffma2(e0, e1, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
                             ffma2(e2, e3, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
-                            w0 += fast_exp2(e0) + fast_exp2(e1);
-                            w1 += fast_exp2(e2) + fast_exp2(e3);
+                            a[0] = fmaf(fast_exp2(e0), r.x, a[0]); a[1] = fmaf(fast_exp2(e1), r.y, a[1]);
+                            a[2] = fmaf(fast_exp2(e2), r.z, a[2]); a[3] = fmaf(fast_exp2(e3), r.w, a[3]);
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const ulonglong2 l = nl[i];
+                            const ulonglong2 l = nm[i];
+                            const float4 r4 = il[i];
+                            const float r[4] = {r4.x, r4.y, r4.z, r4.w};
                             float e[4];
                             ffma2(e[0], e[1], __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
                             ffma2(e[2], e[3], __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) w0 += 64 * h + 4 * i + k >= first ? fast_exp2(e[k]) : 0.f;
+                            for (int k = 0; k < 4; ++k) a[k] = fmaf(64 * h + 4 * i + k >= first ? fast_exp2(e[k]) : 0.f, r[k], a[k]);
                         }
                     }
+                    w += (a[0] + a[1]) + (a[2] + a[3]);
                 }
             }
-            float w = w0 + w1;
             if (KT == 1) {                                       // the two groups share the keys
                 if (grp == 1) s_xch[row] = w;
                 named_bar_sync(1, 256);
