@@ -403,7 +403,8 @@ int launch_flash(battn_handle* h, void* out, float* rec_out, const void* q, cons
         tr::StepMerge T{M, *sv->track, many ? (items + per_block - 1) / per_block : items};
         T.step.hdr = P.hdr; T.step.part = P.part; T.step.scores = P.scores; T.step.cph = P.cph;
         const size_t cum = (size_t)(n_seq + 1) * sizeof(int);
-        const dim3 grid(T.merge_blocks + h->num_sms * (many ? 8 : 2));
+        // (few: what the merge's blocks leave of one wave of two blocks per SM)
+        const dim3 grid(T.merge_blocks + (many ? h->num_sms * 8 : std::max(h->num_sms, 2 * h->num_sms - items)));
         if (many) e = launch_pdl(g.HD == 128 ? tr::k_merge_track_many<128> : tr::k_merge_track_many<256>, grid, dim3(MERGE_M_THREADS), cum, st, T);
         else      e = launch_pdl(g.HD == 128 ? tr::k_merge_track_few<128> : tr::k_merge_track_few<256>, grid, dim3(MERGE_B_THREADS), cum, st, T);
     }

@@ -89,17 +89,15 @@ struct Params {
     float2* stats = nullptr;
     float2* norm = nullptr;
 };
-// the partition (or table row) of a variant's sequence; -1: idle or bad, nothing to do
+// the partition (or table row) of a variant's sequence; -1: idle, -2: bad, nothing to do.  (Without a branch: the caller's
+// early return has to be uniform for the compiler too, or it gives up its uniform registers and spills: 626 -> 598 us for the
+// weight-accumulating call at 512 rows and 32K, 66 -> 61 us for a window chunk with sinks.)
 template <int VAR>
-__device__ __forceinline__ int chunk_slot(const Params& P, bool report) {
+__device__ __forceinline__ int chunk_slot(const Params& P) {
     if (VAR == VAR_PLAIN) return P.slot;
-    if (P.act && P.act[0] == 0) return -1;
     const int s = P.kslot ? P.kslot[0] : P.slot;
-    if (P.kslot && (s < 0 || s >= P.n_slots)) {
-        if (report) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
-        return -1;
-    }
-    return s;
+    const int a = P.act ? P.act[0] : 1;
+    return a == 0 ? -1 : (P.kslot && (s < 0 || s >= P.n_slots) ? -2 : s);
 }
 
 template <int HD, int BN>
@@ -264,6 +262,18 @@ __device__ __forceinline__ void ffma2(float& o0, float& o1, float x0, float x1, 
         : "=f"(o0), "=f"(o1)
         : "f"(x0), "f"(x1), "l"(mul), "l"(add));
 }
+// a running sum of pairs: one add per two terms
+__device__ __forceinline__ void add2(uint64_t& acc, float x, float y) {
+    asm("{\n\t.reg .b64 a;\n\tmov.b64 a, {%1, %2};\n\tadd.rn.f32x2 %0, %0, a;\n\t}" : "+l"(acc) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void scale2(uint64_t& acc, float f) {
+    asm("{\n\t.reg .b64 a;\n\tmov.b64 a, {%1, %1};\n\tmul.rn.f32x2 %0, %0, a;\n\t}" : "+l"(acc) : "f"(f));
+}
+__device__ __forceinline__ float sum2(uint64_t acc) {
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(acc));
+    return x + y;
+}
 template <int N> __device__ __forceinline__ void regs_grow() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_shrink() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -312,8 +322,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         return;
     }
-    const int kv_slot = chunk_slot<VAR>(P, tid == 0);
+    const int kv_slot = chunk_slot<VAR>(P);
     if (VAR != VAR_PLAIN && kv_slot < 0) {                   // (both CTAs of a pair alike)
+        if (kv_slot == -2 && tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         if (early) pdl_wait();                               // a grid that ends before its predecessor breaks the chain of waits
         return;
     }
@@ -326,8 +337,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
     const KeyTiles<VAR, BN> kt(lo_cta, P.sink);
     const int n_all = kt.count(hi_cta);                                // key tiles of this M tile
     const int per_split = (n_all + P.nsplit - 1) / P.nsplit;
-    const int u_first = (int)blockIdx.z * per_split;                   // this CTA's share: tiles kt.at(u_first + j)
+    const int u_first = (int)blockIdx.z * per_split;                   // this CTA's share
     const int n_tiles = max(0, min(per_split, n_all - (int)blockIdx.z * per_split));
+    auto tile_of = [&](int j) { return kt.at(u_first + j); };
     if (n_tiles == 0) {
         // more splits than key tiles (shallow context): an empty record, so the merge ignores this share
         if (early) pdl_wait();
@@ -437,7 +449,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         }
     };
 
-    const size_t hb = ((size_t)(VAR == VAR_PLAIN ? 0 : kv_slot) * P.Hkv + kvh) * P.pstride * (size_t)REC;
+    const size_t hb = (size_t)kvh * P.pstride * (size_t)REC;
 
     if (warp >= (NSOFT + 2 * NDEQ) / 32) regs_shrink<REGS_CTL>();          // the whole last warpgroup
     if (warp == (NSOFT + 2 * NDEQ) / 32) {
@@ -499,7 +511,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
             for (int j = 0; j < n_tiles; ++j) {
                 const int b = j % C::RAW_STAGES;
                 // early streaming stops at the first tile that holds a row of this chunk
-                const int tile = kt.at(u_first + j);
+                const int tile = tile_of(j);
                 if (!waited && (tile + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
                 if (j >= C::RAW_STAGES) wait(B_RAW_FREE0 + b, (j / C::RAW_STAGES - 1) & 1);   // both dequant groups left it
                 const int sp = (tile * BN) & P.ring_mask;
@@ -509,7 +521,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                 // (a paged look-up here is hidden by the ring: the loader runs RAW_STAGES tiles ahead of the dequant warps)
                 const size_t off = P.pg.table ? kv_rec_index(P.pg, kv_slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
                                  : kept ? (((size_t)kv_slot * P.Hkv + kvh) * P.sink.cap + tile * BN) * (size_t)REC
-                                              : hb + (size_t)sp * REC;
+                                              : hb + (VAR == VAR_PLAIN ? 0 : (size_t)kv_slot * P.Hkv * P.pstride * (size_t)REC) + (size_t)sp * REC;
                 uint8_t* dst = RAW + b * 2 * C::RAW_BYTES;
                 mbar_expect_tx(&bars[B_RAW_FULL0 + b], 2 * bytes);
                 bulk_g2s(dst, (kept ? P.sink.k : P.kvk) + off, bytes, &bars[B_RAW_FULL0 + b]);
@@ -532,7 +544,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
 
         for (int j = 0; j < n_tiles; ++j) {
             const int b = j % C::RAW_STAGES;
-            const int t0 = kt.at(u_first + j) * BN;
+            const int t0 = tile_of(j) * BN;
             const uint8_t* Vraw = RAW + b * 2 * C::RAW_BYTES + C::RAW_BYTES;
             wait(B_RAW_FULL0 + b, (j / C::RAW_STAGES) & 1);
             // the P.V MMA that last read this V buffer (tile j - KV_BUFS) must be complete
@@ -637,11 +649,11 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         const float c2 = P.scale_log2;
         const float thr = RESCALE_THRESHOLD / c2;              // threshold in raw-score units
         float m_ref = NEG_BIG;                                 // reference maximum, raw-score units
-        float l_exact = 0.f;                                   // VAR_TRACK: the same sum, of the unrounded weights
+        uint64_t l_exact = 0;                                   // VAR_TRACK: the same sum, of the unrounded weights
         float l_part = 0.f;                                    // this thread's share of sum(P) when the tensor core cannot keep it
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = kt.at(u_first + j) * BN;
+            const int t0 = tile_of(j) * BN;
             const uint32_t tS = tmem + lane_base + ((j & 1) ? C::T_S1 : C::T_S0) + half * HC;
             // tiles every row of the CTA sees completely skip the mask code (bruce.cu:2927-2928)
             // (rows past the end of a ragged M tile hold zero queries: whatever they compute is finite and never stored)
@@ -727,7 +739,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                     }
                     tmem_st_wait();
                 }
-                if (VAR == VAR_TRACK) l_exact *= fast_exp2((m_ref - m_new) * c2);
+                if (VAR == VAR_TRACK) scale2(l_exact, fast_exp2((m_ref - m_new) * c2));
                 m_ref = m_new;
             }
             // p = 2^(s*c2 - m_ref*c2); a row that has seen no key yet keeps the offset at zero, so its hidden
@@ -745,7 +757,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                     float e0, e1;
                     ffma2(e0, e1, __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]), c2p, nbp);
                     e0 = fast_exp2(e0); e1 = fast_exp2(e1);
-                    if (VAR == VAR_TRACK) l_exact += e0 + e1;
+                    if (VAR == VAR_TRACK) add2(l_exact, e0, e1);
                     const uint32_t ph = pack_h2(e0, e1);
                     if constexpr (!C::L_MMA) {
                         // the denominator sums the fp16-rounded weights the MMA multiplies with V, so that
@@ -778,9 +790,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
         if constexpr (VAR == VAR_TRACK) {
             // the other exchange buffer was last read before the barrier above
             volatile float* xch = rmax + ((n_tiles & 1) ^ 1) * 256;
-            xch[half * 128 + m] = l_exact;
+            const float l_own = sum2(l_exact);
+            xch[half * 128 + m] = l_own;
             named_bar_sync(2 + (warp & 3), 64);
-            const float le = l_exact + xch[(half ^ 1) * 128 + m];
+            const float le = l_own + xch[(half ^ 1) * 128 + m];
             const size_t si = ((size_t)blockIdx.z * P.rows + rbase + r) * P.Hq + kvh * G + h;
             const bool some = m_ref > 0.5f * NEG_BIG;
             if (row_ok && half == 0) {

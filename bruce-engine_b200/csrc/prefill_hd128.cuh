@@ -45,8 +45,8 @@
 // Every wait is bounded; a wait that runs out sets the device status word, the remaining waits are
 // skipped, tensor memory is released and the kernel returns.
 // Variants (template parameter VAR, see common.cuh): VAR_SINK walks the sink tiles before the window's; VAR_TRACK also sums the
-// unrounded weights per row (two adds per two exponentials, not measurable beside the plain kernel) for the accumulation
-// in track.cuh.
+// unrounded weights per row (one packed add per two exponentials; 512 rows at 32K: 383 us, plain 359) for the accumulation in
+// track.cuh.
 #pragma once
 #include "prefill.cuh"
 
@@ -192,8 +192,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         return;
     }
-    const int kv_slot = chunk_slot<VAR>(P, tid == 0);
+    const int kv_slot = chunk_slot<VAR>(P);
     if (VAR != VAR_PLAIN && kv_slot < 0) {                   // (both CTAs of a pair alike)
+        if (kv_slot == -2 && tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         if (early) pdl_wait();                               // a grid that ends before its predecessor breaks the chain of waits
         return;
     }
@@ -209,8 +210,9 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     const KeyTiles<VAR, BN> kt(lo_cta, P.sink);
     const int n_all = kt.count(hi_cta);
     const int per_split = (n_all + P.nsplit - 1) / P.nsplit;
-    const int u_first = (int)blockIdx.z * per_split;                          // its tiles: kt.at(u_first + j)
+    const int u_first = (int)blockIdx.z * per_split;
     const int n_tiles = max(0, min(per_split, n_all - (int)blockIdx.z * per_split));
+    auto tile_of = [&](int j) { return kt.at(u_first + j); };
     if (n_tiles == 0) {
         // more splits than key tiles (shallow context): an empty record, so the merge ignores this share
         if (early) pdl_wait();
@@ -338,7 +340,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     auto slot = [](int j) { return j % NB; };
     auto phase = [](int j) { return (uint32_t)((j / NB) & 1); };
 
-    const size_t hb = ((size_t)(VAR == VAR_PLAIN ? 0 : kv_slot) * P.Hkv + kvh) * P.pstride * (size_t)REC;
+    const size_t hb = (size_t)kvh * P.pstride * (size_t)REC;
 
     if (warp >= W_MMA) {
         regs_shrink<REGS_CTL>();                                   // the whole last warpgroup
@@ -412,7 +414,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
             bool waited = !early;
             for (int j = 0; j < n_tiles; ++j) {
                 // early streaming stops at the first tile that holds a row of this chunk
-                const int tile = kt.at(u_first + j);
+                const int tile = tile_of(j);
                 if (!waited && (tile + 1) * BN > p0) { pdl_wait(); pdl_trigger(); waited = true; }
                 if (j >= NB) wait(free_ + slot(j), phase(j - NB), 200);         // the dequant group left it (no hurry: the ring is three deep)
                 const int sp = (tile * BN) & P.ring_mask;
@@ -422,7 +424,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
                 // (a paged look-up here is hidden by the ring: the loader runs three tiles ahead of the dequant warps)
                 const size_t off = P.pg.table ? kv_rec_index(P.pg, kv_slot, kvh, P.Hkv, P.pstride, sp, P.status) * (size_t)REC
                                  : kept ? (((size_t)kv_slot * P.Hkv + kvh) * P.sink.cap + tile * BN) * (size_t)REC
-                                              : hb + (size_t)sp * REC;
+                                              : hb + (VAR == VAR_PLAIN ? 0 : (size_t)kv_slot * P.Hkv * P.pstride * (size_t)REC) + (size_t)sp * REC;
                 mbar_expect_tx(&bars[full + slot(j)], bytes);
                 bulk_g2s(ring + slot(j) * RAW_BYTES, (kept ? (isv ? P.sink.v : P.sink.k) : src) + off, bytes, &bars[full + slot(j)]);
             }
@@ -440,7 +442,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         for (int jj = 0; jj < 8; ++jj) vkey[jj] = kappa(8 * cc + jj);
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = kt.at(u_first + j) * BN;
+            const int t0 = tile_of(j) * BN;
             const uint8_t* Vraw = smem + OFF_RAWV + slot(j) * RAW_BYTES;
             wait(B_VRAW_FULL + slot(j), phase(j), 50);
             // the P.V MMA that last read this V buffer (tile j - NB) must be complete
@@ -552,10 +554,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         // the two threads of a row keep the row reference in a register each: they see the same maxima and take
         // the same decisions
         float m_ref = NEG_BIG;
-        float l_exact = 0.f;                                   // VAR_TRACK: this thread's share of the unrounded weights
+        uint64_t l_exact = 0;                                   // VAR_TRACK: this thread's share of the unrounded weights
 
         for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = kt.at(u_first + j) * BN;
+            const int t0 = tile_of(j) * BN;
             const int ch2 = L::schunk((j ^ 1) < n_tiles);          // the tile's second 32 columns (see Lay::scol)
             const uint32_t tS = tmem + lane_base + T_S + L::scol(slot(j));
             // tiles every row of the CTA sees completely skip the mask code (bruce.cu:2927-2928)
@@ -627,7 +629,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
                     tmem_st_wait();
                     tc_fence_before();
                 }
-                if (VAR == VAR_TRACK && need) l_exact *= fast_exp2((m_ref - m_new) * c2);
+                if (VAR == VAR_TRACK && need) scale2(l_exact, fast_exp2((m_ref - m_new) * c2));
                 if (need) m_ref = m_new;
             }
             // p = 2^(s*c2 - m_ref*c2); a row that has seen no key yet keeps the offset at zero, so its hidden
@@ -643,7 +645,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
                 float e0, e1;
                 ffma2(e0, e1, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), c2p, nbp);
                 e0 = fast_exp2(e0); e1 = fast_exp2(e1);
-                if (VAR == VAR_TRACK) l_exact += e0 + e1;
+                if (VAR == VAR_TRACK) add2(l_exact, e0, e1);
                 pk[i >> 1] = pack_h2(e0, e1);
             }
             tmem_st16(tS + 16 * grp, pk);
@@ -661,9 +663,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         if constexpr (VAR == VAR_TRACK) {
             // the two threads of a row add their shares; the exchange buffer of the opposite tile parity is idle
             volatile float* x = mref + (n_tiles & 1) * 256;
-            x[grp * 128 + m] = l_exact;
+            const float l_own = sum2(l_exact);
+            x[grp * 128 + m] = l_own;
             named_bar_sync(4 + qtr, 64);
-            const float le = l_exact + x[(grp ^ 1) * 128 + m];
+            const float le = l_own + x[(grp ^ 1) * 128 + m];
             const size_t si = ((size_t)blockIdx.z * P.rows + rbase + r) * P.Hq + kvh * G + h;
             const bool some = m_ref > 0.5f * NEG_BIG;
             if (row_ok && grp == 0) {
