@@ -1099,7 +1099,7 @@ static int attend_track_impl(battn_handle* h, void* out, float* score_out, const
         if (ws_bytes < base + tile) return BATTN_ERR_CAPACITY;
         const size_t tiles = (ws_bytes - base) / tile;
         tr::StepParams P{};
-        P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot;
+        P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot; P.act = act; P.status = h->d_status;
         P.n_seq = n_seq; P.Hkv = g.Hkv; P.G = g.G; P.HD = g.HD;
         P.stride = pv ? (size_t)pv->capacity : (size_t)g.slot_ctx;
         StepVariant sv{VAR_TRACK, {}, reinterpret_cast<float*>(w + base), (int)std::min<size_t>(tiles, 0x7fffffff), &P};

@@ -317,15 +317,16 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
     const int kvh = blockIdx.y;
     const bool early = P.early != 0;                        // see Params::early
     if (!early) { pdl_wait(); pdl_trigger(); }
-    const int p0 = P.pos[0];
-    if (p0 < 0 || (!P.is_swa && p0 + P.rows > P.slot_ctx)) {
-        if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
-        return;
-    }
     const int kv_slot = chunk_slot<VAR>(P);
     if (VAR != VAR_PLAIN && kv_slot < 0) {                   // (both CTAs of a pair alike)
         if (kv_slot == -2 && tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         if (early) pdl_wait();                               // a grid that ends before its predecessor breaks the chain of waits
+        return;
+    }
+    const int p0 = P.pos[0];
+    if (p0 < 0 || (!P.is_swa && p0 + P.rows > P.slot_ctx)) {
+        if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
+        if (VAR != VAR_PLAIN && early) pdl_wait();
         return;
     }
     const int rbase = mt * MR;

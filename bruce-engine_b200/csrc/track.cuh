@@ -26,8 +26,10 @@ struct StepParams {
     const float* in;         // score_in, or null: nothing accumulated yet
     const int* pos;
     const int* kslot;
+    const int* act;
     int n_seq, Hkv, G, HD, cph;
     size_t stride;
+    int* status;
 };
 struct StepMerge {           // one launch: blocks below `merge_blocks` merge the outputs, the others accumulate the weights
     MergeParams merge;
@@ -55,7 +57,7 @@ __device__ __forceinline__ float2 item_norm(const StepParams& P, int item, int c
     return make_float2(Mx, 1.f / L);
 }
 
-// Block `cta` of `n_cta` accumulates its contiguous share of the scores' tiles, a thread per position, four in flight.
+// Block `cta` of `n_cta` accumulates its contiguous share of the scores' tiles, a thread per position, several in flight.
 template <int THREADS>
 __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_cta) {
     extern __shared__ int s_cum[];                               // [n_seq + 1]
@@ -73,7 +75,15 @@ __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_c
         const int p = P.pos[pc.i], slot = P.kslot ? P.kslot[pc.i] : 0;
         int clo, chi;
         fd::item_ctas(P.cph, per_cta, P.Hkv, c0, nt, pc.kvh, clo, chi);
-        __syncthreads();                                         // the previous piece has used s_norm
+        // a slot that two active sequences name would get both sums or either one, by chance: neither is written
+        bool twice = false;
+        if (P.kslot)
+            for (int j = tid; j < P.n_seq; j += THREADS) twice |= j != pc.i && P.kslot[j] == slot && !(P.act && P.act[j] == 0);
+        if (__syncthreads_or(twice)) {                           // (and the previous piece has used s_norm)
+            if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
+            g += pc.n;
+            continue;
+        }
         if (warp < P.G) {
             const float2 nm = item_norm(P, pc.i * P.Hkv + pc.kvh, clo, chi, warp, lane);
             if (lane == 0) s_norm[warp] = nm;
@@ -83,7 +93,7 @@ __device__ __forceinline__ void track_step(const StepParams& P, int cta, int n_c
         const float* in = P.in ? P.in + ((size_t)slot * P.Hkv + pc.kvh) * P.stride + first : nullptr;
         float* out = P.out + ((size_t)slot * P.Hkv + pc.kvh) * P.stride + first;
         const float* sc = P.scores + (size_t)g * TILE * P.G;
-        constexpr int UN = 4;
+        constexpr int UN = THREADS == 1024 ? 2 : 4;              // (the big block has 64 registers, and covers 2048 positions)
         if (P.G == 4) {                                          // the usual group: a position's scores are one 16-byte load
             const float2 n0 = s_norm[0], n1 = s_norm[1], n2 = s_norm[2], n3 = s_norm[3];
             for (int k0 = tid; k0 < keys; k0 += UN * THREADS) {

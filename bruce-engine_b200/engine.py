@@ -39,6 +39,7 @@ class AttnEngine:
         if rc:
             raise capi.BattnError("battn_init", rc, self.lib.battn_last_cuda_error(None))
         self.h = h
+        self._ws_need = {}
         self.q_torch = torch.float16 if geom.q_dtype == F16 else torch.float32
         self.out_torch = torch.float16 if geom.out_dtype == F16 else torch.float32
 
@@ -293,14 +294,24 @@ class AttnEngine:
         k, v = (torch.zeros(n.value, dtype=torch.uint8, device=self.device) for _ in range(2))
         return self.sinks(n_sink, k, v), k, v
 
-    def sinks(self, n_sink: int, k=None, v=None):
-        """The descriptor of `n_sink` sinks: over buffers for a ring layer, without for a cache that keeps its first positions."""
+    def sinks(self, n_sink: int, k=None, v=None, cap: int | None = None):
+        """The descriptor of `n_sink` sinks: over the buffers of a ring layer, without for a cache that keeps its first
+        positions.  The buffers are those of all slots; for the single-sequence form (kslot None) one slot's, with `cap`."""
         if (k is None) != (v is None):
             raise ValueError("sinks: both buffers or neither")
         if k is None:
             return capi.CSinks(None, None, n_sink, 0)
-        cap = k.numel() // (self.geom.n_slots * self.geom.n_kv * self.geom.rec)
-        return capi.CSinks(self._dev("k", k, torch.uint8), self._dev("v", v, torch.uint8, k.numel()), n_sink, cap)
+        per = self.geom.n_kv * self.geom.rec
+        n = self.geom.n_slots if cap is None else 1
+        cap = k.numel() // (n * per) if cap is None else cap
+        return capi.CSinks(self._dev("k", k, torch.uint8, n * per * cap), self._dev("v", v, torch.uint8, n * per * cap), n_sink, cap)
+
+    def _part(self, part, n: int, rows: int):
+        """The scratch of an attention call, big enough for it."""
+        need = self._ws_need.get((n, rows))
+        if need is None:
+            need = self._ws_need[n, rows] = self.workspace_bytes(n, rows)
+        return self._dev("part", part, torch.uint8, need)
 
     def sinks_store(self, kvk, kvv, sinks, pos, kslot=None, act=None, rows: int = 1):
         """Behind the append of the same rows: the records of the first positions, ring -> sink buffers."""
@@ -317,14 +328,14 @@ class AttnEngine:
         nq = n * rows * self.geom.n_head * self.geom.head_dim
         self._check("battn_attend_sinks", self.lib.battn_attend_sinks(
             self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), k, v, C.byref(sinks),
-            p, s, a, part.data_ptr(), rows, n, int(is_swa), self._stream_here()))
+            p, s, a, self._part(part, n, rows), rows, n, int(is_swa), self._stream_here()))
 
     def attn_sinks_paged(self, out, q, pages, sinks, pos, part, rows: int = 1, ktab=None, act=None):
         p, s, a, n = self._seqs(pos, ktab, act)
         nq = n * rows * self.geom.n_head * self.geom.head_dim
         self._check("battn_attend_sinks_paged", self.lib.battn_attend_sinks_paged(
             self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), C.byref(pages),
-            C.byref(sinks), p, s, a, part.data_ptr(), rows, n, self._stream_here()))
+            C.byref(sinks), p, s, a, self._part(part, n, rows), rows, n, self._stream_here()))
 
     # ---- attention that accumulates its weights ------------------------------------------------------------
     def alloc_track_part(self, n_seq: int, rows: int, max_positions: int) -> torch.Tensor:
@@ -368,7 +379,7 @@ class AttnEngine:
         d = None if sel_dst is None else self._dev("kslot_dst", sel_dst, torch.int32, n)
         return n, (self._dev("score", score, torch.float32, scores),
                    self._dev("kept", kept, torch.int32, n * self.geom.n_kv * max(budget, 1)),
-                   self._dev("pos_out", pos_out, torch.int32, n), p, s, d, a, part.data_ptr())
+                   self._dev("pos_out", pos_out, torch.int32, n), p, s, d, a, self._dev("part", part, torch.uint8, 4 * n))
 
     def evict(self, kvk, kvv, score, kept, pos_out, pos, part, budget: int, n_sink: int = 0, n_recent: int = 0, kslot=None,
               kslot_dst=None, act=None):

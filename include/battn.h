@@ -371,7 +371,8 @@ int battn_sinks_store(battn_handle* h, const uint8_t* kvk, const uint8_t* kvv, c
  *   rows * (n_head / n_kv) <= 32 and rows <= 8: n_seq sequences, as battn_decode (1 row) and battn_verify
  *   more rows, up to 512: a prompt chunk of one sequence (n_seq = 1), as battn_prefill
  *   q, out [n_seq][rows][n_head][head_dim]; ws: battn_workspace_bytes(n_seq, rows).
- *   kslot / act (ktab) as in those calls; a prompt chunk may name its partition by kslot too.  Sequences with
+ *   kslot / act (ktab) as in those calls; a prompt chunk may name its partition by kslot too.  kslot == NULL: kvk, kvv and
+ *   the sink buffers are the slot's bases.  Sequences with
  *   act[i] == 0 or a bad position produce no output. */
 int battn_attend_sinks(battn_handle* h, void* out, const void* q, const uint8_t* kvk, const uint8_t* kvv,
                        const battn_sinks* sinks, const int* pos, const int* kslot, const int* act, void* ws, int rows,
@@ -389,6 +390,8 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
  * rows of a prompt choose what is kept of it).  score_in may be score_out, but not overlap it otherwise.
  *   score_*  fp32 [slot][kv head][slot_ctx] (paged: [table row][kv head][max_pages * page_len]); with kslot == NULL the
  *            slot's own [kv head][slot_ctx]; 16-byte aligned
+ *   kslot    every active sequence has a slot (or table row) of its own: where two name the same one, the outputs are
+ *            computed, BATTN_DEV_BAD_POSITION is set and neither's scores are written
  *   rows     1: n_seq sequences, one new token each.  2 .. 512: a prompt chunk, or the accepted rows of a speculative
  *            round, of one sequence (n_seq = 1); group a divisor of 128, window >= 64, as battn_prefill
  *   ws       battn_track_workspace_bytes bytes (ws_bytes says how many it has).  The one-row call keeps the scores of every

@@ -131,6 +131,31 @@ def test_no_sinks_equals_the_window_call():
         assert torch.equal(a, b)
 
 
+def test_one_slot_of_a_layer():
+    """The single-sequence form: slot base pointers of the ring and of the sink buffers give what kslot gives."""
+    g = R.geom("B", window=128, slot_ctx=512, n_slots=3)
+    e = R.engine(g)
+    q, k, v = R.draw(g, 700, 60, 21)
+    kr, vr = R.quantised(g, k, v)
+    kvk, kvv = e.alloc_kv_layer(True, fill=0x7F)
+    R.put(e, kvk, {2: (kr, vr)}, True, 0)
+    R.put(e, kvv, {2: (kr, vr)}, True, 1)
+    sk, bk, bv = e.alloc_sinks(130)
+    for buf, r in ((bk, kr), (bv, vr)):
+        buf.view(3, g.n_kv, sk.cap, g.rec)[2].copy_(torch.from_numpy(r[:, :sk.cap].copy()))
+    one = e.sinks(100, bk.view(3, -1)[2], bv.view(3, -1)[2], cap=sk.cap)
+    sk = e.sinks(100, bk, bv)
+    for rows in (1, 8, 60):
+        qd, pos, part = dev_q(e, q[None, :rows]), R.ids([700 - rows], e), e.alloc_part(1, rows)
+        a, b = new_out(e, 1, rows, g.n_head, g.head_dim), new_out(e, 1, rows, g.n_head, g.head_dim)
+        e.attn_sinks(a, qd, kvk, kvv, sk, pos, part, rows=rows, kslot=R.ids([2], e))
+        n = kvk.numel() // 3
+        e.attn_sinks(b, qd, kvk[2 * n:], kvv[2 * n:], one, pos, part, rows=rows)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+        R.assert_attention(to_np(a)[0], R.attend64(g, q[:rows], kr, vr, 700 - rows, 100, 128), g, vr, f"rows {rows}")
+
+
 @pytest.mark.parametrize("early", [False, True])
 def test_a_stream_from_its_first_token(early):
     """Prompt chunk, then single tokens past two windows: append, keep the sinks, attend, in a captured and replayed step;
@@ -258,6 +283,12 @@ def test_refusals():
         call(pos=torch.zeros(1, dtype=torch.int64, device=e.device))
     with pytest.raises(ValueError):
         e.sinks(4, bk)
+    with pytest.raises(ValueError):
+        e.sinks(4, bk, bv, cap=512)                                                # more than the buffers hold
+    with pytest.raises(ValueError):                                                # a scratch buffer for a shorter call
+        e.attn_sinks(torch.empty(1, 100, g.n_head, g.head_dim, dtype=torch.float16, device=e.device),
+                     torch.zeros(1, 100, g.n_head, g.head_dim, dtype=torch.float16, device=e.device), *ring, sk, R.ids([5], e),
+                     part[:4096], rows=100)
     n = __import__("ctypes").c_size_t()
     assert e.lib.battn_sinks_bytes(e.h, 100, n) == capi.ERR_ARG and e.lib.battn_sinks_bytes(e.h, 0, n) == capi.ERR_ARG
     torch.cuda.synchronize()

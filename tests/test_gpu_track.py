@@ -95,6 +95,17 @@ def test_idle_sequences_are_left_alone():
     for name in ("B", "R"):
         for rows in (2, 100):
             _case(name, [600], rows, "paged", 6, "same", act=[0])
+            # what an idle sequence's position and slot hold does not matter
+            g = R.geom(name, slot_ctx=512)
+            e = R.engine(g)
+            q = torch.zeros(1, rows, g.n_head, g.head_dim, dtype=e.q_torch, device=e.device)
+            out, score = new_out(e, 1, rows, g.n_head, g.head_dim), torch.ones(1, g.n_kv, 512, device=e.device)
+            for early in (False, True):
+                e.set_early_kv_stream(early)
+                e.attn_track(out, score, score, q, *e.alloc_kv_layer(False, fill=0), R.ids([-7], e), e.alloc_track_part(1, rows, 512),
+                             rows=rows, kslot=R.ids([99], e), act=R.ids([0], e))
+                torch.cuda.synchronize()
+                assert e.device_status() == 0 and torch.isnan(out).all() and (score == 1).all()
 
 
 def test_attention_output_is_the_plain_calls():
@@ -159,6 +170,66 @@ def test_two_graphs_share_a_workspace_and_repeat():
                 for i, n in enumerate(clean):
                     assert torch.equal(got[i, :, :n], want[i, :, :n])
     assert e.device_status() == 0
+
+
+def test_a_slot_named_twice():
+    """Two active sequences on one slot: both outputs, the status bit, and the slot's scores as they were; the same slot
+    twice is fine when one of the two is idle, and for the others nothing changes."""
+    g = R.geom("B", slot_ctx=512, n_slots=4)
+    e = R.engine(g)
+    kvk, kvv = (torch.randint(0, 60, (e.kv_layer_bytes(False),), dtype=torch.uint8, device=e.device) for _ in range(2))
+    q = torch.randn(3, 1, g.n_head, g.head_dim, device=e.device).half()
+    pos, part = R.ids([300, 200, 100], e), e.alloc_track_part(3, 1, 700)
+    ref, o_ref = torch.full((4, g.n_kv, 512), 5.0, device=e.device), torch.empty_like(q)
+    e.attn_track(o_ref, ref, None, q, kvk, kvv, pos, part, kslot=R.ids([0, 1, 2], e))
+    for slots, act, status in (([1, 1, 2], [1, 1, 1], 1), ([1, 1, 2], [0, 1, 1], 0)):
+        score, o = torch.full_like(ref, 5.0), torch.full_like(q, 9.0)
+        e.attn_track(o, score, None, q, kvk, kvv, pos, part, kslot=R.ids(slots, e), act=R.ids(act, e))
+        torch.cuda.synchronize()
+        assert e.device_status() == status
+        assert torch.equal(o[1:], o_ref[1:]) and torch.equal(score[2], ref[2]) and (score[0] == 5.0).all()
+        assert (score[1] == 5.0).all() if status else torch.equal(score[1], ref[1])
+
+
+def test_the_largest_batch():
+    """1024 sequences of a few positions, ragged, some idle: tracked, attended with sinks, evicted."""
+    g = R.geom("B", slot_ctx=128, n_slots=1024, window=64)
+    e = R.engine(g)
+    rng = np.random.default_rng(8)
+    lens = rng.integers(0, 120, 1024)
+    act = (rng.random(1024) < 0.9).astype(np.int32)
+    q, k, v = R.draw(g, 128, 1, 4)
+    recs = R.quantised(g, k, v)
+    kvk, kvv = e.alloc_kv_layer(False, fill=0)
+    for buf, r in ((kvk, recs[0]), (kvv, recs[1])):
+        buf.copy_(torch.from_numpy(np.broadcast_to(r[None, :, :128], (1024,) + r[:, :128].shape).reshape(-1).copy()))
+    qd = dev_q(e, np.broadcast_to(q[None], (1024,) + q.shape))
+    order = rng.permutation(1024)
+    pos, ks, a = R.ids(lens, e), R.ids(order, e), R.ids(act, e)
+    score = torch.full((1024, g.n_kv, 128), float("nan"), device=e.device)
+    out, out2 = new_out(e, 1024, 1, g.n_head, g.head_dim), new_out(e, 1024, 1, g.n_head, g.head_dim)
+    e.attn_track(out, score, None, qd, kvk, kvv, pos, e.alloc_track_part(1024, 1, int(lens.sum()) + 1024), kslot=ks, act=a)
+    e.attn_sinks(out2, qd, kvk, kvv, e.sinks(4), pos, e.alloc_part(1024, 1), kslot=ks, act=a, is_swa=False)
+    kept, left = torch.full((1024, g.n_kv, 40), -9, dtype=torch.int32, device=e.device), R.ids([-9] * 1024, e)
+    torch.cuda.synchronize()
+    sc = score.cpu().numpy()
+    e.evict(kvk, kvv, score, kept, left, pos, e.alloc_evict_part(1024), 40, n_sink=2, n_recent=8, kslot=ks, act=a)
+    torch.cuda.synchronize()
+    assert e.device_status() == 0
+    got, got2, kept, left = to_np(out), to_np(out2), kept.cpu().numpy(), left.cpu().numpy()
+    for i in range(0, 1024, 7):
+        p = int(lens[i])
+        if not act[i]:
+            assert np.isnan(got[i]).all() and np.isnan(got2[i]).all() and left[i] == -9 and (kept[i] == -9).all()
+            continue
+        R.assert_attention(got[i], R.attend64(g, q, *recs, p), g, recs[1], f"track {i}")
+        R.assert_attention(got2[i], R.attend64(g, q, *recs, p, 4, 64), g, recs[1], f"sinks {i}")
+        want = R.score64(g, q, recs[0], p, None)
+        R.assert_scores(sc[order[i], :, :p + 1], want, g, q, recs[0], p, f"scores {i}")
+        assert left[i] == min(p, 40)
+        for h in range(g.n_kv):
+            idx = R.evict_list(sc[order[i], h, :p], 40, 2, 8)
+            assert (kept[i, h, :len(idx)] == idx).all() and (kept[i, h, len(idx):] == -1).all()
 
 
 def test_a_workspace_that_is_too_small_for_the_positions():
