@@ -104,6 +104,14 @@ cudaError_t fd_prepare_all(battn_handle* h) {
     }
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_TRACK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(tr::k_track_chunk<HD>, tr::ChunkCfg<HD>::SMEM)) != cudaSuccess) return e;
+    {
+        void* f = nullptr;                                      // the driver's encoder, without linking against the driver
+        cudaDriverEntryPointQueryResult found;
+        e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
+        if (e != cudaSuccess) return e;
+        if (found != cudaDriverEntryPointSuccess || !f) return cudaErrorNotSupported;
+        h->encode_tiled = reinterpret_cast<decltype(h->encode_tiled)>(f);
+    }
     if ((e = allow_smem(ev::k_evict_select<1024>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_select<512>, ev::KEYS_SMEM * 4)) != cudaSuccess) return e;
     if ((e = allow_smem(ev::k_evict_move<HD>, ev::MoveCfg<HD>::ROUND_MAX * ev::MoveCfg<HD>::PER)) != cudaSuccess) return e;
@@ -1112,12 +1120,22 @@ static int attend_track_impl(battn_handle* h, void* out, float* score_out, const
         if (g.W < 64) return BATTN_ERR_ARG;                     // as battn_prefill
         ChunkVariant cv{VAR_TRACK, kslot, act, {}, reinterpret_cast<float2*>(w + cw.stats), reinterpret_cast<float2*>(w + cw.norm)};
         if ((rc = launch_prefill(h, out, q, kvk, kvv, pos, ws, rows, 0, st, nullptr, pv, 0, &cv))) return rc;
-        tr::ChunkParams P;
+        tr::ChunkParams P{};
         P.q = q; P.kvk = kvk; P.norm = cv.norm; P.out = score_out; P.in = score_in; P.pos = pos; P.kslot = kslot; P.act = act;
         P.rows = rows; P.Hq = g.Hq; P.Hkv = g.Hkv; P.G = g.G; P.q_f16 = g.q_f16;
         P.pstride = pv ? pv->capacity : g.slot_ctx; P.n_slots = pv ? pv->n_tables : g.n_slots;
         P.scale_log2 = g.scale * LOG2E; P.status = h->d_status;
         if (pv) P.pg = pv->pg;
+        if (g.q_f16) {
+            // (rank 3; the strides in bytes are those of head and row)
+            const cuuint64_t dims[3] = {(cuuint64_t)g.HD, (cuuint64_t)g.Hq, (cuuint64_t)rows};
+            const cuuint64_t strides[2] = {(cuuint64_t)g.HD * 2, (cuuint64_t)g.Hq * g.HD * 2};
+            const cuuint32_t box[3] = {64, (cuuint32_t)g.G, (cuuint32_t)(tr::QN / g.G)}, step[3] = {1, 1, 1};
+            const CUresult r = h->encode_tiled(&P.q_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box,
+                                               step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            if (r != CUDA_SUCCESS) return cuda_fail(h, cudaErrorInvalidValue);
+        }
         const dim3 grid(h->num_sms), block(tr::CTHREADS);
         e = g.HD == 128 ? launch_pdl(tr::k_track_chunk<128>, grid, block, tr::ChunkCfg<128>::SMEM, st, P)
                         : launch_pdl(tr::k_track_chunk<256>, grid, block, tr::ChunkCfg<256>::SMEM, st, P);

@@ -1,5 +1,6 @@
 // Shared declarations of the attention library: geometry, the handle, PTX helpers.
 #pragma once
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -40,6 +41,7 @@ struct battn_handle {
     int vw_ctas_per_sm;      // resident CTAs per SM of the wide verify kernel
     int fd_ctas_per_sm[3];   // resident CTAs per SM of the flash-decode kernel, per NT in {1,2}
     int fd_smem[3];
+    decltype(&cuTensorMapEncodeTiled) encode_tiled;   // the driver's, looked up by battn_init
     int evict_clusters;      // clusters of the eviction's move that are resident at one CTA per SM
     // Early KV streaming of the decode kernels (see fd::Params::early): allowed for a call when the last launch on
     // this handle wrote no cache rows other than the call's own (kvw_kind 0: none, 1: rows_per_seq rows at kvw_pos of

@@ -8,6 +8,8 @@
 // in the same launch.
 // k_track_chunk, a prompt chunk: the scores are formed a second time; only K is read.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 #include "exact.cuh"
 #include "prefill.cuh"
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_track_many(const Step
 }
 
 struct ChunkParams {
+    CUtensorMap q_map;       // fp16 queries [row][head][dim], boxes of 128 / G rows x G heads x 64 dims, 128-byte swizzle
     const void* q;
     const uint8_t* kvk;
     const float2* norm;      // [row][head]: (m, 1 / l)
@@ -178,7 +181,15 @@ struct ChunkParams {
 // 512 rows at 32K, 32/8 heads of 128: 245 us at 1.6 GHz (warp MMAs with scales on fp32 sums took 705, the divisions 390);
 // exponentials 62 % of their rate, tensor pipe 60 %.
 constexpr int QN = 128;                     // pairs per Q tile
-constexpr int CTHREADS = 14 * 32;           // warps 0-7 convert K and sum weights, 8-11 load Q, 12 issues the MMAs, 13 loads K
+
+// one box of a 3-d tensor map into shared memory (no multicast); x is a multiple of 64 halves
+__device__ __forceinline__ void tensor_g2s(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+constexpr int W_Q = 8, W_MMA = 10, W_K = 11;
+constexpr int CTHREADS = 12 * 32;           // warps 0-7 convert K and sum weights, 8-9 load Q, 10 issues the MMAs, 11 loads K
 constexpr int MAX_PAIRS = MAX_PREFILL * 8;
 
 template <int HD>
@@ -202,7 +213,7 @@ struct ChunkCfg {
 enum { B_RAWF = 0, B_RAWE = 1, B_KRDY = 2, B_QF = 3, B_QE = 7, B_DF = 11, B_DE = 13, N_CBARS = 15 };
 
 template <int HD>
-__global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P) {
+__global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const __grid_constant__ ChunkParams P) {
     using namespace pf;
     using C = ChunkCfg<HD>;
     constexpr int NBLK = C::NBLK, REC = C::REC, KT = C::KT, QST = C::QST;
@@ -223,12 +234,12 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
     if ((int)blockIdx.x >= units) return;
     if (tid == 0) {
         mbar_init(&bars[B_RAWF], 1); mbar_init(&bars[B_RAWE], 8); mbar_init(&bars[B_KRDY], 8);
-        for (int i = 0; i < QST; ++i) { mbar_init(&bars[B_QF + i], 4); mbar_init(&bars[B_QE + i], 1); }
+        for (int i = 0; i < QST; ++i) { mbar_init(&bars[B_QF + i], P.q_f16 ? 1 : W_MMA - W_Q); mbar_init(&bars[B_QE + i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_DF + i], 1); mbar_init(&bars[B_DE + i], 4); }
         misc[1] = 0;
         mbar_fence_init();
     }
-    if (warp == 12) {
+    if (warp == W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(const_cast<uint32_t*>(&misc[0]))), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -310,46 +321,33 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
                 // pairs of this tile that see the key: index at least (key - p0) G
                 const int first = (key - p0) * G - qt * QN;
                 const bool masked = t0 + C::KEYS - 1 > p0 + qt * QN / G;
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t v[64];
-                    tmem_ld32_nowait(tD + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-                    tmem_ld32_nowait(tD + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-                    tmem_ld_wait();
-                    if (h == 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bars[B_DE + grp]);
-                    }
-                    const ulonglong2* nm = reinterpret_cast<const ulonglong2*>(s_nm + qt * QN + 64 * h);
-                    const float4* il = reinterpret_cast<const float4*>(s_il + qt * QN + 64 * h);
-                    float a[4] = {0.f, 0.f, 0.f, 0.f};           // sums of 16 terms each: what a long sum would round away
-                    if (!masked) {
+// the whole accumulator into registers, so that the next product can have it back before the exponentials
+                uint32_t v[128];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const ulonglong2 l = nm[i];
-                            const float4 r = il[i];
-                            float e0, e1, e2, e3;
-                            ffma2(e0, e1, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
-                            ffma2(e2, e3, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
-                            a[0] = fmaf(fast_exp2(e0), r.x, a[0]); a[1] = fmaf(fast_exp2(e1), r.y, a[1]);
-                            a[2] = fmaf(fast_exp2(e2), r.z, a[2]); a[3] = fmaf(fast_exp2(e3), r.w, a[3]);
-                        }
-                    } else {
+                for (int c = 0; c < 4; ++c) tmem_ld32_nowait(tD + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[B_DE + grp]);
+                const ulonglong2* nm = reinterpret_cast<const ulonglong2*>(s_nm + qt * QN);
+                const float4* il = reinterpret_cast<const float4*>(s_il + qt * QN);
+                float a[4] = {0.f, 0.f, 0.f, 0.f};               // sums of 32 terms each: what a long sum would round away
+                if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const ulonglong2 l = nm[i];
-                            const float4 r4 = il[i];
-                            const float r[4] = {r4.x, r4.y, r4.z, r4.w};
-                            float e[4];
-                            ffma2(e[0], e[1], __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
-                            ffma2(e[2], e[3], __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) a[k] = fmaf(64 * h + 4 * i + k >= first ? fast_exp2(e[k]) : 0.f, r[k], a[k]);
-                        }
-                    }
-                    w += (a[0] + a[1]) + (a[2] + a[3]);
+                    for (int i = 0; i < 128; ++i)
+                        if (i < first) v[i] = __float_as_uint(-INFINITY);
                 }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const ulonglong2 l = nm[i];
+                    const float4 r = il[i];
+                    float e0, e1, e2, e3;
+                    ffma2(e0, e1, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), c2p, l.x);
+                    ffma2(e2, e3, __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]), c2p, l.y);
+                    a[0] = fmaf(fast_exp2(e0), r.x, a[0]); a[1] = fmaf(fast_exp2(e1), r.y, a[1]);
+                    a[2] = fmaf(fast_exp2(e2), r.z, a[2]); a[3] = fmaf(fast_exp2(e3), r.w, a[3]);
+                }
+                w += (a[0] + a[1]) + (a[2] + a[3]);
             }
             if (KT == 1) {                                       // the two groups share the keys
                 if (grp == 1) s_xch[row] = w;
@@ -362,58 +360,53 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
                 P.out[at] = w;
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < W_MMA) {
         // ======================= Q tiles: [pair][dim], 64-dim sub-tiles, 128-byte swizzle ================================
-        const int t = tid - 256;
         uint32_t cnt = 0;
-        auto load = [&](int kvh, int qt, uint32_t c) {
-            // thread t: 16-byte chunk `ch` of every PSTEP-th pair
-            constexpr int PSTEP = 128 / (HD / 8);
-            const int ch = t & (HD / 8 - 1), pr0 = t / (HD / 8);
-            uint8_t* dst = smem + (c % QST) * C::Q_BYTES + (ch >> 3) * C::Q_SUB;
-#pragma unroll 8
-            for (int pr = pr0; pr < QN; pr += PSTEP) {
-                const int pair = qt * QN + pr;
-                uint8_t* to = dst + sw128(pr, ch & 7);
-                if (pair < pairs) {
-                    const size_t qi = ((size_t)(pair >> lg) * P.Hq + kvh * G + (pair & (G - 1))) * HD + ch * 8;
-                    if (P.q_f16) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)),
-                                     "l"(reinterpret_cast<const __half*>(P.q) + qi) : "memory");
-                    } else {
-                        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + qi);
-                        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + qi + 4);
-                        *reinterpret_cast<uint4*>(to) = make_uint4(pack_h2(x.x, x.y), pack_h2(x.z, x.w), pack_h2(y.x, y.y), pack_h2(y.z, y.w));
+        if (P.q_f16) {
+            // one box of the queries' tensor map per sub-tile: 128 / G rows of G heads of 64 dims, zeros past the last row
+            if (warp == W_Q && lane == 0) {
+                for (int u = blockIdx.x; u < units; u += gridDim.x) {
+                    const int kvh = u % P.Hkv;
+                    for (int qt = unit_qt0(unit_t0(u)); qt < n_qt; ++qt, ++cnt) {
+                        const int st = cnt % QST;
+                        if (cnt >= QST) wait(B_QE + st, (cnt / QST - 1) & 1);
+                        mbar_expect_tx(&bars[B_QF + st], C::Q_BYTES);
+#pragma unroll
+                        for (int sub = 0; sub < HD / 64; ++sub)
+                            tensor_g2s(smem + st * C::Q_BYTES + sub * C::Q_SUB, &P.q_map, 64 * sub, kvh * G, qt * (QN >> lg), &bars[B_QF + st]);
                     }
-                } else {
-                    *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        auto publish = [&](uint32_t c) {                         // tile c has landed: hand it to the tensor core's proxy
-            proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[B_QF + c % QST]);
-        };
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
-            const int t0 = unit_t0(u);
-            for (int qt = unit_qt0(t0); qt < n_qt; ++qt, ++cnt) {
-                if (QST == 2 && cnt > 0) {                       // a ring of two: the tile before must go first
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    publish(cnt - 1);
-                }
-                if (cnt >= QST) wait(B_QE + cnt % QST, (cnt / QST - 1) & 1);
-                load(u % P.Hkv, qt, cnt);
-                if (QST > 2 && cnt > 0) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    publish(cnt - 1);
+        } else {
+            // fp32 queries are rounded on the way: thread t has 16-byte chunk `ch` of every PSTEP-th pair
+            constexpr int PSTEP = (W_MMA - W_Q) * 32 / (HD / 8);
+            const int t = tid - W_Q * 32, ch = t & (HD / 8 - 1), pr0 = t / (HD / 8);
+            for (int u = blockIdx.x; u < units; u += gridDim.x) {
+                const int kvh = u % P.Hkv;
+                for (int qt = unit_qt0(unit_t0(u)); qt < n_qt; ++qt, ++cnt) {
+                    const int st = cnt % QST;
+                    if (cnt >= QST) wait(B_QE + st, (cnt / QST - 1) & 1);
+                    uint8_t* dst = smem + st * C::Q_BYTES + (ch >> 3) * C::Q_SUB;
+#pragma unroll 4
+                    for (int pr = pr0; pr < QN; pr += PSTEP) {
+                        const int pair = qt * QN + pr;
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (pair < pairs) {
+                            const float* src = reinterpret_cast<const float*>(P.q) +
+                                               ((size_t)(pair >> lg) * P.Hq + kvh * G + (pair & (G - 1))) * HD + ch * 8;
+                            const float4 x = *reinterpret_cast<const float4*>(src), y = *reinterpret_cast<const float4*>(src + 4);
+                            w = make_uint4(pack_h2(x.x, x.y), pack_h2(x.z, x.w), pack_h2(y.x, y.y), pack_h2(y.z, y.w));
+                        }
+                        *reinterpret_cast<uint4*>(dst + sw128(pr, ch & 7)) = w;
+                    }
+                    proxy_fence();                               // hand it to the tensor core's proxy
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars[B_QF + st]);
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        publish(cnt - 1);
-    } else if (warp == 12) {
+    } else if (warp == W_MMA) {
         // ======================= the products ============================================================================
         if (lane == 0) {
             const uint32_t id = umma_idesc(128, QN);
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const ChunkParams P
         }
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == W_MMA) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
