@@ -170,16 +170,18 @@ struct ChunkParams {
 // Persistent CTAs, one per SM; a unit is (kv head, 256 keys at head_dim 128, 128 keys at 256).  S^T = K Q^T on tcgen05 with
 // 128 keys on the M side, so that a TMEM lane is a key and the sum over the rows is a sum over columns, inside one thread.
 //   * K is the tensor-memory A operand and stays there for the unit, in two exact fp16 parts like in the prompt kernels
-//     (hi = fp16(d x), lo = d x - hi): the scores carry no rounding of K.  From shared memory it would be read again by
-//     every product, and a 128-column product with both operands there runs into the shared-memory bandwidth.
-//   * Q tiles of 128 (row, head) pairs stream from L2 through a ring as the B operand; every one serves all keys of the unit
-//     (two M tiles at head_dim 128: half the L2 traffic, which at one would be near 7 TB/s).
-//   * Two accumulators of 128 columns; each of two groups of four warps empties its own: w += 2^(s c - m) / l, one exponential
-//     per score.  The exponentials (16 per cycle and SM) take as long as the two products: that balance is the bound.
+//     (hi = fp16(d x), lo = d x - hi): the scores carry no rounding of K.  (From shared memory the products run as
+//     fast -- 64 cycles for 128 x 128 x 16 either way -- but its 128 KB are the Q ring's.)
+//   * Q tiles of 128 (row, head) pairs stream from L2 through a ring as the B operand, by tiled copies that place them swizzled;
+//     every one serves all keys of the unit (two M tiles at head_dim 128: half the L2 traffic, which at one would be near 7 TB/s).
+//     Loader warps did this before and were the bound: with divisions 390 us, with shifts 245, copies 236.  (fp32 queries are
+//     still brought by warps, which round them.)
+//   * Two accumulators of 128 columns; each of two groups of four warps takes its own into registers whole, frees it, and adds up
+//     w += 2^(s c - m) / l, one exponential per score.  The exponentials (16 per cycle and SM) take as long as the two products:
+//     that balance is the bound.
 //   * Between units the eight warps convert the next K, whose raw records were fetched ahead.
-//   * The Q loader shifts instead of dividing (the group is a power of two): with divisions it was the bound.
-// 512 rows at 32K, 32/8 heads of 128: 245 us at 1.6 GHz (warp MMAs with scales on fp32 sums took 705, the divisions 390);
-// exponentials 62 % of their rate, tensor pipe 60 %.
+// 512 rows at 32K, 32/8 heads of 128: 236 us (warp MMAs with scales on fp32 sums took 705) at 1.61 GHz, which is what the power cap
+// leaves; exponentials 64 % of their rate, tensor pipe 62 %.  A quarter or half of the exponentials on the FMA pipes: no gain.
 constexpr int QN = 128;                     // pairs per Q tile
 
 // one box of a 3-d tensor map into shared memory (no multicast); x is a multiple of 64 halves

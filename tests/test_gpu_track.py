@@ -172,6 +172,94 @@ def test_two_graphs_share_a_workspace_and_repeat():
     assert e.device_status() == 0
 
 
+def test_offsets_past_32_bits():
+    """The last slot of a 5.7 GB cache (and of pages as far) gives what slot 0 gives: weights, sinks and eviction."""
+    from bruce_engine_b200 import capi
+    g = R.geom("B", slot_ctx=262144, n_slots=20, window=128)
+    e = R.engine(g)
+    kvk, kvv = (e.alloc_kv_layer(False)[0] for _ in range(2))
+    assert kvk.numel() > 2 ** 32
+    for rows in (1, 40):
+        q, k, v = R.draw(g, 500 + rows, rows, rows)
+        recs = R.quantised(g, k, v)
+        for buf, r in ((kvk, recs[0]), (kvv, recs[1])):
+            for s in (0, 19):
+                buf.view(20, g.n_kv, -1, g.rec)[s, :, :500 + rows].copy_(torch.from_numpy(r.copy()))
+        qd, pos = dev_q(e, q[None]), R.ids([500], e)
+        score = torch.zeros(20, g.n_kv, g.slot_ctx, device=e.device)
+        res = {}
+        # pages of 128: the whole cache seen as a pool, page p of the row at the pool's end or start
+        n_pages = kvk.numel() // (g.n_kv * 128 * g.rec)
+        for s in (0, 19):
+            out, out2 = new_out(e, 1, rows, g.n_head, g.head_dim), new_out(e, 1, rows, g.n_head, g.head_dim)
+            kept, left = torch.zeros(1, g.n_kv, 200, dtype=torch.int32, device=e.device), R.ids([0], e)
+            slot = R.ids([s], e)
+            e.attn_track(out, score, score, qd, kvk, kvv, pos, e.alloc_track_part(1, rows, 600), rows=rows, kslot=slot)
+            e.attn_sinks(out2, qd, kvk, kvv, e.sinks(4), pos, e.alloc_part(1, rows), rows=rows, kslot=slot, is_swa=False)
+            e.evict(kvk, kvv, score, kept, left, pos, e.alloc_evict_part(1), 200, n_recent=50, kslot=slot)
+            res[s] = [out, out2, kept, left, score[s, :, :200].clone(),
+                      kvk.view(20, g.n_kv, -1, g.rec)[s, :, :200].clone(), kvv.view(20, g.n_kv, -1, g.rec)[s, :, :200].clone()]
+        for s, first in ((0, 0), (19, n_pages - 6)):
+            tab = torch.arange(first, first + 5, dtype=torch.int32, device=e.device)[None].contiguous()
+            for buf, r in ((kvk, recs[0]), (kvv, recs[1])):
+                pool = buf[:n_pages * g.n_kv * 128 * g.rec].view(n_pages, g.n_kv, 128, g.rec)
+                for p in range(5):
+                    x = torch.from_numpy(r[:, 128 * p:128 * (p + 1)].copy())
+                    pool[first + p, :, :x.shape[1]].copy_(x)
+            desc = capi.CPages(kvk.data_ptr(), kvv.data_ptr(), tab.data_ptr(), n_pages, 1, 5, 128)
+            out, sc = new_out(e, 1, rows, g.n_head, g.head_dim), torch.zeros(1, g.n_kv, 640, device=e.device)
+            e.attn_track_paged(out, sc, None, qd, desc, pos, e.alloc_track_part(1, rows, 600), rows=rows)
+            res[s] += [out, sc]
+        torch.cuda.synchronize()
+        assert e.device_status() == 0
+        for a, b in zip(res[0], res[19]):
+            assert torch.equal(a, b)
+        R.assert_attention(to_np(res[19][0])[0], R.attend64(g, q, *recs, 500), g, recs[1], "far slot")
+        assert torch.equal(res[19][0], res[19][7])
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams, each with its own buffers and scratch, on one handle: what each computes alone."""
+    g = R.geom("B", slot_ctx=8192, n_slots=2)
+    e = R.engine(g)
+
+    def job(seed):
+        torch.manual_seed(seed)
+        kv = [torch.randint(0, 60, (e.kv_layer_bytes(False),), dtype=torch.uint8, device=e.device) for _ in range(2)]
+        q1 = torch.randn(2, 1, g.n_head, g.head_dim, device=e.device).half()
+        q2 = torch.randn(1, 200, g.n_head, g.head_dim, device=e.device).half()
+        o1, o2, s = torch.empty_like(q1), torch.empty_like(q2), torch.zeros(2, g.n_kv, 8192, device=e.device)
+        part, ep = e.alloc_track_part(2, 200, 16384), e.alloc_evict_part(2)
+        kept, left = torch.zeros(2, g.n_kv, 3000, dtype=torch.int32, device=e.device), R.ids([0, 0], e)
+        pos, ks = R.ids([7000, 6000], e), R.ids([0, 1], e)
+
+        def run():
+            e.attn_track(o1, s, s, q1, *kv, pos, part, kslot=ks)
+            e.attn_track(o2, s, s, q2, *kv, pos[1:], part, rows=200, kslot=ks[1:])
+            e.evict(*kv, s, kept, left, pos, ep, 3000, n_sink=4, n_recent=100, kslot=ks)
+            e.attn_track(o1, s, s, q1, *kv, left, part, kslot=ks)
+        return run, [o1, o2, s, kept, left] + kv
+
+    alone = []
+    for seed in (1, 2):
+        run, got = job(seed)
+        run()
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in got])
+    for _ in range(3):
+        jobs = [job(seed) for seed in (1, 2)]
+        streams = [torch.cuda.Stream() for _ in jobs]
+        torch.cuda.synchronize()
+        for (run, _), st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                run()
+        torch.cuda.synchronize()
+        assert e.device_status() == 0
+        for (_, got), want in zip(jobs, alone):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
 def test_a_slot_named_twice():
     """Two active sequences on one slot: both outputs, the status bit, and the slot's scores as they were; the same slot
     twice is fine when one of the two is idle, and for the others nothing changes."""
