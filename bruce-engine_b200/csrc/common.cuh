@@ -246,6 +246,7 @@ __device__ __forceinline__ SeqRange seq_range(const int* __restrict__ pos, const
 // sequence of a ring layer, where the ring has replaced them; every tile below cap is read from them, those of a young
 // sequence too.  k == nullptr: a cache that still holds its first positions, read in place.
 constexpr int SINK_TILE = 128;              // cap is a multiple of the widest key tile
+constexpr int SINK_MAX_POS = 0x7fffffff - 1024;   // first rows on a ring up to here: the tiles behind them still count in 32 bits
 struct SinkView {
     const uint8_t* k = nullptr;
     const uint8_t* v = nullptr;
@@ -260,7 +261,13 @@ __device__ __forceinline__ SeqRange seq_keys(const int* __restrict__ pos, const 
                                              const int* __restrict__ act, int i, int rows, int is_swa, int W, int slot_ctx,
                                              int n_slots, int* status) {
     SeqRange s = seq_range(pos, kslot, act, i, rows, is_swa, W, slot_ctx, n_slots, status);
-    if (VAR == VAR_SINK && s.active) s.lo = max(0, s.p0 + 1 - W);
+    if (VAR == VAR_SINK && s.active) {
+        s.lo = max(0, s.p0 + 1 - W);
+        if (s.p0 > SINK_MAX_POS) {
+            atomicOr(status, BATTN_DEV_BAD_POSITION);
+            s.active = false; s.lo = s.hi = 0;
+        }
+    }
     return s;
 }
 

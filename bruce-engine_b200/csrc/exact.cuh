@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(MERGE_M_THREADS) k_merge_chunk(const MergePara
     const int warp = blockIdx.x * (MERGE_M_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int item = warp / PARTS, d0 = warp % PARTS * (HD / PARTS);
     const size_t items = (size_t)P.n_rows * P.Hq;
-    if (!sr.active || item >= (int)items) return;
+    if (!sr.active || sr.p0 > SINK_MAX_POS || item >= (int)items) return;
     const float* base = P.part + (size_t)item * (HD + 2);
     const size_t stride = items * (HD + 2);
     const float2 ml = lane < P.count ? *reinterpret_cast<const float2*>(base + lane * stride + HD) : make_float2(NEG_BIG, 0.f);

@@ -194,7 +194,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         return;
     }
     const int p0 = P.pos[0];
-    if (p0 < 0 || (!P.is_swa && p0 + P.rows > P.slot_ctx)) {
+    if (p0 < 0 || (!P.is_swa && p0 + P.rows > P.slot_ctx) || (VAR == VAR_SINK && p0 > SINK_MAX_POS)) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         if (VAR != VAR_PLAIN && early) pdl_wait();
         return;

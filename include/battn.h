@@ -355,7 +355,7 @@ int battn_attend_exact_paged(battn_handle* h, void* out, const void* q, const ba
  *     EVERY key below cap is read from the sink buffers, those of a sequence that still fits the ring too.
  *   - a full layer (is_swa = 0) and a paged cache: the first positions are where they always were; k = v = NULL.  Page
  *     table entries of pages that lie wholly between the sinks and the window are never read and may be -1.
- * n_sink is 0 .. window. */
+ * n_sink is 0 .. window; first rows stand at positions up to 2^31 - 1025. */
 typedef struct battn_sinks {
     uint8_t* k;
     uint8_t* v;

@@ -247,6 +247,62 @@ def test_an_unmapped_page_that_is_needed_sets_the_status_bit():
             assert e.device_status() == status, (rows, page)
 
 
+def test_positions_at_the_end_of_32_bits():
+    """A ring's positions only grow: the last ones the call takes, and those it refuses."""
+    g = R.geom("B", window=128, slot_ctx=512)
+    e = R.engine(g)
+    last = 2 ** 31 - 1025
+    for rows in (1, 8, 100):
+        q, k, v = R.draw(g, 256, rows, rows)
+        kr, vr = R.quantised(g, k, v)
+        # the ring's 256 slots, and sinks from another time; what the rows see is put in order for the plain form
+        kvk, kvv = e.alloc_kv_layer(True, fill=0)
+        sk, bk, bv = e.alloc_sinks(4)
+        for buf, s, r in ((kvk, bk, kr), (kvv, bv, vr)):
+            buf.view(g.n_kv, 256, g.rec).copy_(torch.from_numpy(r.copy()))
+            s.view(g.n_kv, sk.cap, g.rec)[:, :4].copy_(torch.from_numpy(r[:, 100:104].copy()))
+        out = new_out(e, 1, rows, g.n_head, g.head_dim)
+        part = e.alloc_part(1, rows)
+        e.attn_sinks(out, dev_q(e, q[None]), kvk, kvv, sk, R.ids([last], e), part, rows=rows)
+        torch.cuda.synchronize()
+        assert e.device_status() == 0
+        seen = np.r_[100:104, (np.arange(last + 1 - 128, last + rows) % 256)]
+        # 4 sinks, then 128 + rows - 1 keys of the ring: rows at positions 4 + 127 ... of that sequence, window 128
+        want = R.attend64(g, q, kr[:, seen], vr[:, seen], 131, 4, 128)
+        R.assert_attention(to_np(out)[0], want, g, vr, f"rows {rows}")
+        out = new_out(e, 1, rows, g.n_head, g.head_dim)
+        e.attn_sinks(out, dev_q(e, q[None]), kvk, kvv, sk, R.ids([last + 1], e), part, rows=rows)
+        torch.cuda.synchronize()
+        assert e.device_status() == 1 and torch.isnan(out).all()
+
+
+def test_a_capacity_that_ends_inside_a_tile():
+    """slot_ctx need only be even: the last tile of a partition is shorter, and what follows is another slot's."""
+    g = R.geom("B", window=128, slot_ctx=634, n_slots=3)
+    for name in ("B", "R"):
+        g = R.geom(name, window=128, slot_ctx=634, n_slots=3)
+        e = R.engine(g)
+        for rows in (1, 8, 34):
+            p = 634 - rows
+            q, k, v = R.draw(g, 634, rows, rows)
+            recs = R.quantised(g, k, v)
+            kvk, kvv = e.alloc_kv_layer(False, fill=0x7F)
+            for buf, t in ((kvk, 0), (kvv, 1)):
+                R.put(e, buf, {1: recs}, False, t)
+            qd, pos, slot = dev_q(e, q[None]), R.ids([p], e), R.ids([1], e)
+            out, out2 = new_out(e, 1, rows, g.n_head, g.head_dim), new_out(e, 1, rows, g.n_head, g.head_dim)
+            e.attn_sinks(out, qd, kvk, kvv, e.sinks(70), pos, e.alloc_part(1, rows), rows=rows, kslot=slot, is_swa=False)
+            score = torch.full((3, g.n_kv, 634), 5.0, device=e.device)
+            e.attn_track(out2, score, None, qd, kvk, kvv, pos, e.alloc_track_part(1, rows, 634), rows=rows, kslot=slot)
+            torch.cuda.synchronize()
+            assert e.device_status() == 0
+            R.assert_attention(to_np(out)[0], R.attend64(g, q, *recs, p, 70, 128), g, recs[1], f"sinks {name} {rows}")
+            R.assert_attention(to_np(out2)[0], R.attend64(g, q, *recs, p), g, recs[1], f"track {name} {rows}")
+            sc = score.cpu().numpy()
+            R.assert_scores(sc[1], R.score64(g, q, recs[0], p, None), g, q, recs[0], p, f"scores {name} {rows}")
+            assert (sc[[0, 2]] == 5.0).all()
+
+
 def test_refusals():
     from bruce_engine_b200 import capi
     g = R.geom("B", window=128, slot_ctx=512, n_slots=2)
