@@ -125,6 +125,14 @@ cudaError_t fd_prepare_all(battn_handle* h) {
         cfg.dynamicSmemBytes = ev::MoveCfg<HD>::ROUND_MAX * ev::MoveCfg<HD>::PER;
         if ((e = cudaOccupancyMaxActiveClusters(&h->evict_clusters, ev::k_evict_move<HD>, &cfg)) != cudaSuccess) return e;
     }
+    // the others are loaded here too, so that a call's first time may be a capture
+    const void* small[] = {(const void*)k_sinks_store, (const void*)k_merge_many<HD>, (const void*)k_merge_chunk<HD, 1>,
+                           (const void*)k_merge_chunk<HD, HD / 64>, (const void*)tr::k_merge_track_few<HD>,
+                           (const void*)tr::k_merge_track_many<HD>};
+    for (const void* f : small) {
+        cudaFuncAttributes a;
+        if ((e = cudaFuncGetAttributes(&a, f)) != cudaSuccess) return e;
+    }
     if ((e = allow_smem(vw::k_verify_wide<HD, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 1, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;
     if ((e = allow_smem(fd::k_flash_decode<HD, 2, 0, VAR_SINK>, SMEM_MAX)) != cudaSuccess) return e;

@@ -218,6 +218,48 @@ def test_offsets_past_32_bits():
         assert torch.equal(res[19][0], res[19][7])
 
 
+def test_a_first_call_may_be_captured():
+    """In a fresh process every new call is captured before it ever ran, then replayed."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from tests import bounded_ref as R
+for name in ("B", "R16"):
+    g = R.geom(name, window=128, slot_ctx=2048, n_slots=20)
+    e = R.engine(g)
+    kv = [torch.randint(0, 60, (e.kv_layer_bytes(False),), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    ring = e.alloc_kv_layer(True, fill=0)
+    sk, bk, bv = e.alloc_sinks(4)
+    q = {r: torch.randn(r, g.n_head, g.head_dim, device="cuda").half() for r in (1, 8, 20, 90)}
+    o = {r: torch.zeros_like(x) for r, x in q.items()}
+    s = torch.zeros(20, g.n_kv, 2048, device="cuda")
+    pos, ks = R.ids([900] * 20, e), R.ids(range(20), e)
+    part, tp, ep = e.alloc_part(20, 90), e.alloc_track_part(20, 90, 40000), e.alloc_evict_part(20)
+    kept, left = torch.zeros(20, g.n_kv, 300, dtype=torch.int32, device="cuda"), R.ids([0] * 20, e)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        e.sinks_store(*ring, sk, pos[:1], kslot=ks[:1])
+        for r in (1, 8, 90):
+            e.attn_sinks(o[r], q[r], *kv, e.sinks(4), pos[:1], part, rows=r, kslot=ks[:1], is_swa=False)
+        e.attn_sinks(o[20], q[20], *kv, e.sinks(4), pos, part, kslot=ks, is_swa=False)
+        e.attn_track(o[1], s, s, q[1], *kv, pos[:1], tp, kslot=ks[:1])
+        e.attn_track(o[20], s, s, q[20], *kv, pos, tp, kslot=ks)
+        e.attn_track(o[90], s, s, q[90], *kv, pos[:1], tp, rows=90, kslot=ks[:1])
+        e.evict(*kv, s, kept, left, pos, ep, 300, kslot=ks)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert e.device_status() == 0 and left.tolist() == [300] * 20 and all(torch.isfinite(x).all() for x in o.values())
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
 def test_calls_on_two_streams_at_once():
     """Two streams, each with its own buffers and scratch, on one handle: what each computes alone."""
     g = R.geom("B", slot_ctx=8192, n_slots=2)
