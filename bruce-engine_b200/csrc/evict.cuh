@@ -18,7 +18,7 @@ constexpr int MAX_CLUSTER = 8;              // the portable limit
 constexpr int MOVE_THREADS = 512;           // 256 where several CTAs share an SM
 constexpr int KEYS_SMEM = 40 * 1024;        // keys a CTA keeps in shared memory at most (160 KB); a longer share re-reads the rest
 // Candidates that are worth another CTA of the cluster: up to here a pass over them is shorter than the cluster barriers
-// (4160 positions, one CTA of eight: 23 -> 12 us)
+// (4160 positions, one CTA of eight: 23 -> 10 us)
 constexpr int KEYS_PER_CTA = 8192;
 constexpr int MATCHES = 2048;               // keys of the first pass's bin that are listed
 
@@ -133,7 +133,7 @@ __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_
 }
 
 // SEL_THREADS: 1024 for few clusters, where a pass over the keys is the time; 512 once they outnumber the SMs, so that three
-// CTAs share one (32 sequences of up to 8192: 20 -> 13 us)
+// CTAs share one (32 sequences of up to 8192: 20 -> 14 us)
 template <int SEL_THREADS>
 __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_select(const Params P) {
     extern __shared__ __align__(16) uint32_t s_key[];            // P.keys keys of this CTA's share
@@ -271,9 +271,9 @@ __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_selec
 }
 
 // A round of a CTA: P.round records, chosen by the host: all of the CTA's part in one round when there are few clusters (the
-// SM has the room, and a round costs two trips to memory one after the other: 4096 records of 272 bytes, 15 -> 9 us),
+// SM has the room, and a round costs two trips to memory one after the other: 4096 records of 272 bytes, 15 -> 11 us),
 // half of it where the clusters would not all be resident at one CTA per SM (about nine of eight CTAs are: 16 clusters of 151 KB
-// ran in two waves, 22 us instead of 14), otherwise 34 KB, so that several CTAs share an SM and two buffers overlap the rounds.
+// ran in two waves, 22 us instead of 19), otherwise 34 KB, so that several CTAs share an SM and two buffers overlap the rounds.
 template <int HD>
 struct MoveCfg {
     static constexpr int REC = HD + HD / 16, WORDS = REC / 8;
