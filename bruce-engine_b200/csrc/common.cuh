@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/battn.h"
+#include "work_cut.h"
 
 namespace battn {
 
@@ -225,10 +226,10 @@ __device__ __forceinline__ SeqRange seq_range(const int* __restrict__ pos, const
     s.active = act ? (act[i] != 0) : true;
     s.slot = kslot ? kslot[i] : 0;
     s.p0 = pos[i];
-    s.lo = is_swa ? max(0, s.p0 + 1 - W) : 0;
-    s.hi = s.p0 + rows;
+    s.lo = is_swa ? max(0, (int)(s.p0 + 1u - W)) : 0;            // (unsigned: a position that is refused below may wrap)
+    s.hi = (int)((unsigned)s.p0 + rows);
     if (s.active) {
-        const bool bad = s.p0 < 0 || (!is_swa && s.hi > slot_ctx) || s.slot < 0 || (kslot && s.slot >= n_slots);
+        const bool bad = !rows_fit(s.p0, rows, is_swa != 0, slot_ctx) || s.slot < 0 || (kslot && s.slot >= n_slots);
         if (bad) {
             atomicOr(status, BATTN_DEV_BAD_POSITION);
             s.active = false;

@@ -194,7 +194,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
         return;
     }
     const int p0 = P.pos[0];
-    if (p0 < 0 || (!P.is_swa && p0 + P.rows > P.slot_ctx) || (VAR == VAR_SINK && p0 > SINK_MAX_POS)) {
+    if (!rows_fit(p0, P.rows, P.is_swa != 0, P.slot_ctx) || (VAR == VAR_SINK && p0 > SINK_MAX_POS)) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
         if (VAR != VAR_PLAIN && early) pdl_wait();
         return;
@@ -215,9 +215,10 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     const int n_tiles = max(0, min(per_split, n_all - (int)blockIdx.z * per_split));
     auto tile_of = [&](int j) { return kt.at(u_first + j); };
     if (n_tiles == 0) {
-        // more splits than key tiles (shallow context): an empty record, so the merge ignores this share
+        // more splits than key tiles (shallow context): an empty record, so the merge ignores this share (one split always
+        // has a tile, and has no records)
         if (early) pdl_wait();
-        if (tid < 128 && tid / G < rows_eff) {
+        if (P.recs && tid < 128 && tid / G < rows_eff) {
             float* rec = P.recs + ((((size_t)blockIdx.z * P.rows) + rbase + tid / G) * P.Hq + kvh * G + tid % G) * (size_t)(HD + 2);
             for (int i = 0; i < HD; ++i) rec[i] = 0.f;
             rec[HD] = NEG_BIG; rec[HD + 1] = 0.f;

@@ -1,5 +1,6 @@
-// The work cut of the split-K attention kernels (flash-decode, both verify kernels) and the matching record ranges of
-// the merge kernel: plain integer logic, shared by device code and by a host test (tests/host/cut_test.cpp).
+// The work cut of the split-K attention kernels (flash-decode, both verify kernels), the matching record ranges of the
+// merge kernel, and the check of a sequence's positions that comes before both: plain integer logic, shared by device code
+// and by host tests (tests/host/cut_test.cpp, position_test.cpp).
 //
 // Work unit = (sequence, kv head, tile); `cum[i]` = tiles per kv head of the sequences before i.  Tiles are numbered
 // g = Hkv * cum[i] + kvh * nt_i + t.  A CTA owns tiles [g0, g1); the tiles of one (sequence, kv head) item inside a
@@ -13,6 +14,17 @@
 #endif
 
 namespace battn {
+
+// May the rows of a sequence stand at positions p0 .. p0 + rows - 1 of a cache of `cap` positions (`ring`: of any length)?
+// Asked without p0 + rows, which wraps for positions a stray word can hold: a wrapped end passes for a short sequence, whose
+// negative tile count sends the other sequences' records out of the workspace.  POS_ROOM keeps what the kernels form
+// behind the last row, the end of its key tile, in 32 bits as well.
+constexpr int POS_ROOM = 256;               // the widest key tile or unit of tiles
+BATTN_HD bool rows_fit(int p0, int rows, bool ring, int cap) {
+    const int end = 0x7fffffff - POS_ROOM;
+    return p0 >= 0 && p0 <= (ring || cap > end ? end : cap) - rows;
+}
+
 namespace fd {
 
 struct Piece {

@@ -54,7 +54,8 @@ enum { BATTN_F32 = 0, BATTN_F16 = 1 };
 
 /* bits of the device status word (battn_device_status) */
 enum {
-    BATTN_DEV_BAD_POSITION = 1,  /* a row's position fell outside the cache; the row was skipped  */
+    BATTN_DEV_BAD_POSITION = 1,  /* a row's position fell outside the cache; the row was skipped (attention calls: the
+                                  * sequence; on a ring its rows end at 2^31 - 257 at the latest) */
     BATTN_DEV_WAIT_TIMEOUT = 2,  /* a bounded in-kernel wait ran out; results of that launch void */
     BATTN_DEV_WORKSPACE    = 4   /* battn_attend_track: more cached positions than ws has room for; call skipped */
 };
