@@ -196,7 +196,7 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
     const int p0 = P.pos[0];
     if (!rows_fit(p0, P.rows, P.is_swa != 0, P.slot_ctx) || (VAR == VAR_SINK && p0 > SINK_MAX_POS)) {
         if (tid == 0) atomicOr(P.status, BATTN_DEV_BAD_POSITION);
-        if (VAR != VAR_PLAIN && early) pdl_wait();
+        if (early) pdl_wait();                               // (as above)
         return;
     }
     const int rbase = max(mt, 0) * MR;

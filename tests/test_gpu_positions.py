@@ -119,3 +119,33 @@ def test_the_other_sequences_of_a_batch(rows):
             assert torch.isnan(got[0][0][[1, 4]]).all() and torch.isfinite(got[0][0][[0, 2, 3, 5]]).all()
             for x, y in zip(*got):
                 assert torch.equal(torch.nan_to_num(x, nan=7.0), torch.nan_to_num(y, nan=7.0)), (i, far)
+
+
+@pytest.mark.parametrize("name", ["B", "R"])
+def test_a_refused_prompt_chunk_keeps_the_order_of_the_stream(name):
+    """With early streaming, append -> chunk that ends past the cache -> decode over the rows that were appended: the refused
+    chunk's launches still stand behind the append, so the decode reads its rows, as without early streaming."""
+    cap, rows = 4096, 512
+    g = R.geom(name, window=1024, slot_ctx=cap)
+    e = R.engine(g)
+    rng = np.random.default_rng(3)
+    q1, qc = (dev_q(e, rng.standard_normal((1, r, g.n_head, g.head_dim)).astype(np.float32)) for r in (1, rows))
+    kvk, kvv = e.alloc_kv_layer(False, fill=1)
+    part, first, last = e.alloc_part(1, rows), R.ids([cap - 400], e), R.ids([cap - 1], e)
+    junk = new_out(e, 1, rows, g.n_head, g.head_dim)
+    for t in range(20):
+        kv = torch.randn(2, rows, g.n_kv, g.head_dim, device=e.device)
+        got = []
+        for early in (True, False):
+            kvk.fill_(1)
+            kvv.fill_(1)
+            torch.cuda.synchronize()
+            out = new_out(e, 1, 1, g.n_head, g.head_dim)
+            e.set_early_kv_stream(early)
+            e.qkv_prep_store(kv[0], kv[1], kvk, kvv, first, rows=rows)
+            e.launch_attn_m(junk, qc, kvk, kvv, first, part, rows)
+            e.launch_attn_m(out, q1, kvk, kvv, last, part, 1)
+            torch.cuda.synchronize()
+            assert e.device_status() == BAD
+            got.append(out)
+        assert torch.isfinite(got[0]).all() and torch.equal(*got), t
