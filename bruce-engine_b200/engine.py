@@ -344,6 +344,10 @@ class AttnEngine:
                     self.lib.battn_track_workspace_bytes(self.h, n_seq, rows, max_positions, C.byref(n)))
         return torch.empty(n.value, dtype=torch.uint8, device=self.device)
 
+    def _track_part(self, part):
+        """Pointer and bytes of the scratch of a weight-accumulating call; the library checks that they suffice."""
+        return self._dev("part", part, part.dtype), part.numel() * part.element_size()
+
     def _track_args(self, out, score_out, score_in, q, rows, n, scores):
         nq = n * rows * self.geom.n_head * self.geom.head_dim
         return (self._dev("out", out, self.out_torch, nq), self._dev("score_out", score_out, torch.float32, scores),
@@ -358,15 +362,14 @@ class AttnEngine:
         k, v = self._cache_ptrs(kvk, kvv, False, kslot is not None)
         args = self._track_args(out, score_out, score_in, q, rows, n, (1 if kslot is None else g.n_slots) * g.n_kv * g.slot_ctx)
         self._check("battn_attend_track", self.lib.battn_attend_track(
-            self.h, *args, k, v, p, s, a, part.data_ptr(), part.numel() * part.element_size(), rows, n, self._stream_here()))
+            self.h, *args, k, v, p, s, a, *self._track_part(part), rows, n, self._stream_here()))
 
     def attn_track_paged(self, out, score_out, score_in, q, pages, pos, part, rows: int = 1, ktab=None, act=None):
         p, s, a, n = self._seqs(pos, ktab, act)
         args = self._track_args(out, score_out, score_in, q, rows, n, (1 if ktab is None else pages.n_tables) *
                                 self.geom.n_kv * pages.max_pages * pages.page_len)
         self._check("battn_attend_track_paged", self.lib.battn_attend_track_paged(
-            self.h, *args, C.byref(pages), p, s, a, part.data_ptr(), part.numel() * part.element_size(), rows, n,
-            self._stream_here()))
+            self.h, *args, C.byref(pages), p, s, a, *self._track_part(part), rows, n, self._stream_here()))
 
     # ---- eviction by accumulated attention weight --------------------------------------------------------
     def alloc_evict_part(self, n_seq: int) -> torch.Tensor:
