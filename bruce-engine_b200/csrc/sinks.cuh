@@ -36,8 +36,8 @@ __global__ void __launch_bounds__(256) k_sinks_store(const SinkStoreParams P) {
     const uint2* src = reinterpret_cast<const uint2*>((blockIdx.z ? P.kvv : P.kvk) + head * P.ring * P.rec);
     uint2* dst = reinterpret_cast<uint2*>((blockIdx.z ? P.sv : P.sk) + head * P.cap * P.rec);
     for (int w = threadIdx.x; w < n * wpr; w += blockDim.x) {
-        const int r = w / wpr, c = w - r * wpr, p = p0 + r;
-        dst[p * wpr + c] = src[(size_t)(p & (P.ring - 1)) * wpr + c];
+        const int r = w / wpr, c = w - r * wpr, p = p0 + r;      // (below cap; its words may pass 32 bits)
+        dst[(size_t)p * wpr + c] = src[(size_t)(p & (P.ring - 1)) * wpr + c];
     }
 }
 
