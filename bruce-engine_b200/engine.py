@@ -304,7 +304,15 @@ class AttnEngine:
         per = self.geom.n_kv * self.geom.rec
         n = self.geom.n_slots if cap is None else 1
         cap = k.numel() // (n * per) if cap is None else cap
-        return capi.CSinks(self._dev("k", k, torch.uint8, n * per * cap), self._dev("v", v, torch.uint8, n * per * cap), n_sink, cap)
+        d = capi.CSinks(self._dev("k", k, torch.uint8, n * per * cap), self._dev("v", v, torch.uint8, n * per * cap), n_sink, cap)
+        d.slots = min(k.numel(), v.numel()) // max(per * cap, 1)
+        return d
+
+    def _sinks(self, sinks, kslot):
+        """The descriptor for a call; partitions are named by kslot only over buffers that have one for every slot."""
+        if kslot is not None and getattr(sinks, "slots", self.geom.n_slots) < self.geom.n_slots:
+            raise ValueError(f"sinks: buffers of {sinks.slots} of {self.geom.n_slots} slots in a call that names slots")
+        return C.byref(sinks)
 
     def _part(self, part, n: int, rows: int):
         """The scratch of an attention call, big enough for it."""
@@ -317,8 +325,8 @@ class AttnEngine:
         """Behind the append of the same rows: the records of the first positions, ring -> sink buffers."""
         p, s, a, n = self._seqs(pos, kslot, act)
         k, v = self._cache_ptrs(kvk, kvv, True, kslot is not None)
-        self._check("battn_sinks_store", self.lib.battn_sinks_store(self.h, k, v, C.byref(sinks), p, s, a, n, rows,
-                                                                    self._stream_here()))
+        self._check("battn_sinks_store", self.lib.battn_sinks_store(self.h, k, v, self._sinks(sinks, kslot), p, s, a,
+                                                                    n, rows, self._stream_here()))
 
     def attn_sinks(self, out, q, kvk, kvv, sinks, pos, part, rows: int = 1, kslot=None, act=None, is_swa: bool = True):
         """Sliding-window attention whose rows see the first n_sink positions too: `rows` rows of every sequence (decode,
@@ -327,8 +335,8 @@ class AttnEngine:
         k, v = self._cache_ptrs(kvk, kvv, is_swa, kslot is not None)
         nq = n * rows * self.geom.n_head * self.geom.head_dim
         self._check("battn_attend_sinks", self.lib.battn_attend_sinks(
-            self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), k, v, C.byref(sinks),
-            p, s, a, self._part(part, n, rows), rows, n, int(is_swa), self._stream_here()))
+            self.h, self._dev("out", out, self.out_torch, nq), self._dev("q", q, self.q_torch, nq), k, v,
+            self._sinks(sinks, kslot), p, s, a, self._part(part, n, rows), rows, n, int(is_swa), self._stream_here()))
 
     def attn_sinks_paged(self, out, q, pages, sinks, pos, part, rows: int = 1, ktab=None, act=None):
         p, s, a, n = self._seqs(pos, ktab, act)
