@@ -11,6 +11,7 @@ torch is used only for device memory and streams; every computation is a call in
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -98,10 +99,25 @@ class AttnEngine:
             self.h, _ptr(k), _ptr(v), _ptr(kvk), _ptr(kvv), _ptr(pos), _ptr(kslot), _ptr(act),
             n_seq, rows, int(is_swa), self._stream()))
 
-    def kv_copy_prefix(self, kvk, kvv, src_slot: int, dst_slot: int, n_pos: int, is_swa: bool = False):
-        """Prefix sharing between slots: the first n_pos cached positions of src_slot copied into dst_slot."""
+    def kv_copy_prefix(self, kvk, kvv, src_slot: int, dst_slot: int, n_pos: int, is_swa: bool = False, sinks=None, score=None):
+        """Prefix sharing between slots: the first n_pos cached positions of src_slot copied into dst_slot, and with them what
+        the layer keeps beside its records: a window layer's sink buffers (`sinks`, a descriptor over buffers of all slots) or a
+        full layer's accumulated scores (`score` [slot][n_kv][slot_ctx])."""
+        g = self.geom
+        if sinks is not None and (not is_swa or getattr(sinks, "slots", 0) < g.n_slots):
+            raise ValueError("kv_copy_prefix: sinks are a window layer's, over buffers of all slots made by sinks() or alloc_sinks()")
+        if score is not None:
+            if is_swa:
+                raise ValueError("kv_copy_prefix: scores are a full layer's")
+            self._dev("score", score, torch.float32, g.n_slots * g.n_kv * g.slot_ctx)
         self._check("battn_kv_copy_prefix", self.lib.battn_kv_copy_prefix(
             self.h, _ptr(kvk), _ptr(kvv), src_slot, dst_slot, n_pos, int(is_swa), self._stream()))
+        beside = [] if score is None else [(score, (g.slot_ctx,), n_pos)]
+        if sinks is not None:
+            beside += [(b, (sinks.cap, g.rec), min(n_pos, sinks.cap)) for b in sinks.bufs]
+        for buf, shape, n in beside:
+            x = buf.reshape(-1)[:g.n_slots * g.n_kv * math.prod(shape)].view(g.n_slots, g.n_kv, *shape)
+            x[dst_slot, :, :n].copy_(x[src_slot, :, :n])
 
     def qkv_prep(self, q_out, q, k, v, sqk, cs, sn, kvk, kvv, pos, kslot=None, act=None, rows: int = 1,
                  is_swa: bool = False, theta_sel: int = 1):
@@ -305,7 +321,7 @@ class AttnEngine:
         n = self.geom.n_slots if cap is None else 1
         cap = k.numel() // (n * per) if cap is None else cap
         d = capi.CSinks(self._dev("k", k, torch.uint8, n * per * cap), self._dev("v", v, torch.uint8, n * per * cap), n_sink, cap)
-        d.slots = min(k.numel(), v.numel()) // max(per * cap, 1)
+        d.slots, d.bufs = min(k.numel(), v.numel()) // max(per * cap, 1), (k, v)
         return d
 
     def _sinks(self, sinks, kslot):

@@ -125,7 +125,13 @@ int battn_kv_append(battn_handle* h, const float* k, const float* v, uint8_t* kv
  * (Session::cache_hit, engine/src/session.h:337-346, with the slot chosen by affinity, server.h:376-396); with its
  * contiguous per-slot partitions (bruce.cu:5471-5503) sharing across slots is a copy, and this is that copy.
  * kvk, kvv: the LAYER base pointers.  On a sliding-window layer the ring slots of the last min(n_pos, 2*window)
- * positions are copied.  Bytes are copied verbatim: the destination's records equal the source's. */
+ * positions are copied.  Bytes are copied verbatim: the destination's records equal the source's.
+ * Only records are copied.  What a layer keeps beside them stays with the slot and is the host's to copy with the prefix:
+ *   sink buffers (battn_sinks): positions [0, min(n_pos, cap)) of every kv head, K and V -- without them the rows attend to the
+ *       sinks of the slot's previous sequence, which a ring past them no longer holds;
+ *   accumulated scores (battn_attend_track): positions [0, n_pos) of every kv head, or zeros to count from here on.
+ * Each is one strided copy per buffer on `stream` (cudaMemcpy2DAsync, a row per kv head).  Scores go with a prefix of shared
+ * pages in the same way, from table row to table row. */
 int battn_kv_copy_prefix(battn_handle* h, uint8_t* kvk, uint8_t* kvv, int src_slot, int dst_slot, int n_pos, int is_swa,
                          void* stream);
 
@@ -353,7 +359,8 @@ int battn_attend_exact_paged(battn_handle* h, void* out, const void* q, const ba
  *         k, v: [slot][kv head][cap positions][record], battn_sinks_bytes each, cap a multiple of 128, >= n_sink
  *     which hold the first `cap` positions of every sequence.  battn_sinks_store copies them from the ring; call it after
  *     every append until the sequence is longer than cap (later calls do nothing, so it may stay in a captured step).
- *     EVERY key below cap is read from the sink buffers, those of a sequence that still fits the ring too.
+ *     EVERY key below cap is read from the sink buffers, those of a sequence that still fits the ring too; a sequence that starts
+ *     behind a copied prefix needs its sink buffers copied as well (battn_kv_copy_prefix).
  *   - a full layer (is_swa = 0) and a paged cache: the first positions are where they always were; k = v = NULL.  Page
  *     table entries of pages that lie wholly between the sinks and the window are never read and may be -1.
  * n_sink is 0 .. window; first rows stand at positions up to 2^31 - 1025. */
@@ -387,7 +394,8 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
  *     out as battn_decode / battn_prefill,
  *     score_out[kv head][p] = (p < pos[i] ? score_in[kv head][p] : 0) + sum over rows r and heads h of w[r][h][p]
  * for p <= pos[i]+rows-1; positions past them are not touched, and the call's own positions start from nothing, so the
- * buffers need no clearing when a slot begins a new sequence.  score_in == NULL: nothing was accumulated before (the last
+ * buffers need no clearing when a slot begins a new sequence at position 0.  One that begins behind a prefix -- copied,
+ * on shared pages, or the slot's own -- adds to the scores that stand at the prefix's positions: copy the prefix's, or zero them.  score_in == NULL: nothing was accumulated before (the last
  * rows of a prompt choose what is kept of it).  score_in may be score_out, but not overlap it otherwise.
  *   score_*  fp32 [slot][kv head][slot_ctx] (paged: [table row][kv head][max_pages * page_len]); with kslot == NULL the
  *            slot's own [kv head][slot_ctx]; 16-byte aligned

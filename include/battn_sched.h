@@ -134,7 +134,8 @@ public:
         return true;
     }
     /* The empty row `dst` starts with the pages that hold the first n_pos positions of `src`; only whole pages are
-     * shared.  Returns the number of positions dst now holds (a multiple of the page length). */
+     * shared.  Returns the number of positions dst now holds (a multiple of the page length).  Scores that
+     * battn_attend_track accumulates belong to the row, not to its pages: copy those of the shared positions (or zero them). */
     int share_prefix(int src, int dst, int n_pos) {
         if (used_[(size_t)dst] != 0) return 0;
         int n = std::min(n_pos / page_len_, used_[(size_t)src]);
