@@ -352,9 +352,14 @@ int battn_attend_exact_paged(battn_handle* h, void* out, const void* q, const ba
 /* ---- Sliding window with sinks -------------------------------------------------------------------------------------
  * A row at position p sees its window and the first n_sink positions of its sequence:
  *     key <= p  and  (key > p - window  or  key < n_sink)
- * (no counterpart in the reference, whose window layers forget their first tokens).  A model that was trained with full
- * attention keeps its quality over an endless stream when the first few tokens, which draw most of the attention no row
- * needs elsewhere, stay visible beside the window.  The geometry's window applies.  Three kinds of cache:
+ * (no counterpart in the reference, whose window layers forget their first tokens): the first few tokens, which draw much of
+ * the attention that no row needs elsewhere, stay visible beside the window.  Records keep the rotation they were stored with,
+ * so a row's rotary distance to the sinks grows with the stream; the published use of sinks with models trained on full
+ * attention counts positions inside the cache instead (keys are rotated when they are read), which is not done here.  Whether
+ * a model holds its quality past the distances it was trained on is the host's to know.
+ * Accuracy: as the calls it stands beside (battn_decode, battn_verify, battn_prefill).  Scores and sums are fp32; the weights and
+ * the values d * x enter the second product as fp16 each, which puts fp16 outputs about 3.5e-4 (2-norm) from 64 bits.
+ * The geometry's window applies.  Three kinds of cache:
  *   - a ring layer (is_swa = 1): the ring forgets the first positions, so they are kept in sink buffers beside it,
  *         k, v: [slot][kv head][cap positions][record], battn_sinks_bytes each, cap a multiple of 128, >= n_sink
  *     which hold the first `cap` positions of every sequence.  battn_sinks_store copies them from the ring; call it after
@@ -407,7 +412,9 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
  *            position there: max_positions bounds the sum over the active sequences of the positions they hold, the new ones
  *            included.  A call that meets more sets BATTN_DEV_WORKSPACE and writes nothing.
  * The weights divide by a denominator that is summed in fp32 from unrounded weights (the output divides by the sum of the
- * fp16 weights its product uses); fp32 queries are rounded to fp16 first, as everywhere.  No atomics: results repeat. */
+ * fp16 weights its product uses); fp32 queries are rounded to fp16 first, as everywhere.  Measured distance of the scores from 64
+ * bits (2-norm, fp16 queries): one row 2e-7 to 4e-7; a chunk, whose scores are formed on the tensor core, 1e-6 to 3e-6 at
+ * head_dim 128 and 3e-6 to 6e-6 at 256.  No atomics: results repeat. */
 int battn_track_workspace_bytes(const battn_handle* h, int n_seq, int rows_per_seq, long long max_positions, size_t* out_bytes);
 int battn_attend_track(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q, const uint8_t* kvk,
                        const uint8_t* kvv, const int* pos, const int* kslot, const int* act, void* ws, size_t ws_bytes, int rows,
