@@ -469,13 +469,15 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill(const Params P) {
                     wait(B_KF0 + hf, j & 1);
                     tc_fence_after();
                     // S += Q_half K_hi^T + Q_half K_lo^T: the two fp16 parts add up to the exact product d * x of
-                    // every cached value, so the scores carry no rounding of the K operand
+                    // every cached value, so the scores carry no rounding of the K operand.  (VAR_TRACK: the low part
+                    // first, see track.cuh)
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                    for (int turn = 0; turn < 2; ++turn)
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
+                            const int part = VAR == VAR_TRACK ? 1 - turn : turn;
                             const uint64_t b = umma_desc(ka + hf * C::K_HALF_BYTES + part * C::K_PART_BYTES + (ks >> 2) * (BN * 128)) + 2 * (ks & 3);
-                            umma_f16_ts(d, tmem + C::T_Q + 8 * (8 * hf + ks), b, idS, (hf | part | ks) != 0);
+                            umma_f16_ts(d, tmem + C::T_Q + 8 * (8 * hf + ks), b, idS, (hf | turn | ks) != 0);
                         }
                     umma_commit(&bars[B_KFREE0 + hf]);          // the dequant warps may refill this half
                 }

@@ -371,18 +371,19 @@ __global__ void __maxnreg__(REGS_LAUNCH) k_prefill_hd128(const Params P) {
                 const uint64_t kd = kd0 + (uint64_t)(L::koff(slot(j), 0) >> 4);
                 const uint64_t kl = kl0 + (uint64_t)(L::koff(slot(j), 0) >> 4);
                 // S = Q K_hi^T + Q K_lo^T: the two fp16 parts add up to the exact product d * x of every cached
-                // value, so the scores carry no rounding of the K operand
+                // value, so the scores carry no rounding of the K operand.  (VAR_TRACK: the low part first, see track.cuh)
+                const uint64_t k1 = VAR == VAR_TRACK ? kl : kd, k2 = VAR == VAR_TRACK ? kd : kl;
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint64_t off = (uint64_t)((ks >> 2) * sub_step + 2 * (ks & 3));
-                    if (PAIR) umma2_f16_ts(d, tmem + T_Q + 8 * ks, kd + off, id, ks > 0);
-                    else      umma_f16_ts(d, tmem + T_Q + 8 * ks, kd + off, id, ks > 0);
+                    if (PAIR) umma2_f16_ts(d, tmem + T_Q + 8 * ks, k1 + off, id, ks > 0);
+                    else      umma_f16_ts(d, tmem + T_Q + 8 * ks, k1 + off, id, ks > 0);
                 }
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint64_t off = (uint64_t)((ks >> 2) * sub_step + 2 * (ks & 3));
-                    if (PAIR) umma2_f16_ts(d, tmem + T_Q + 8 * ks, kl + off, id, 1u);
-                    else      umma_f16_ts(d, tmem + T_Q + 8 * ks, kl + off, id, 1u);
+                    if (PAIR) umma2_f16_ts(d, tmem + T_Q + 8 * ks, k2 + off, id, 1u);
+                    else      umma_f16_ts(d, tmem + T_Q + 8 * ks, k2 + off, id, 1u);
                 }
                 if (PAIR) {
                     umma2_commit(&bars[B_S + slot(j)]);

@@ -172,6 +172,11 @@ struct ChunkParams {
 //   * K is the tensor-memory A operand and stays there for the unit, in two exact fp16 parts like in the prompt kernels
 //     (hi = fp16(d x), lo = d x - hi): the scores carry no rounding of K.  (From shared memory the products run as
 //     fast -- 64 cycles for 128 x 128 x 16 either way -- but its 128 KB are the Q ring's.)
+//     The low part comes first, here and in the attention kernel's VAR_TRACK instances: every accumulation step drops what
+//     lies below the running sum's 24 bits, always towards zero, so that large scores lose, and the low part's steps are
+//     free of it only while the sum is small.  (Distance of the weights from 64 bits, 2-norm, 2 rows at 16000 positions: head_dim
+//     128 2.7e-6 -> 1.3e-6, 256 6.1e-6 -> 1.0e-6.  At 256 the attention kernel takes the dims in two halves; the same order here,
+//     low, high, low, high, gave 3.0e-6.)
 //   * Q tiles of 128 (row, head) pairs stream from L2 through a ring as the B operand, by tiled copies that place them swizzled;
 //     every one serves all keys of the unit (two M tiles at head_dim 128: half the L2 traffic, which at one would be near 7 TB/s).
 //     Loader warps did this before and were the bound: with divisions 390 us, with shifts 245, copies 236.  (fp32 queries are
@@ -429,11 +434,11 @@ __global__ void __launch_bounds__(CTHREADS, 1) k_track_chunk(const __grid_consta
                         tc_fence_after();
                         const uint32_t d = tmem + C::T_D + b * 128, ka = tmem + kt * HD;
 #pragma unroll
-                        for (int part = 0; part < 2; ++part)
+                        for (int part = 1; part >= 0; --part)    // the low part first, see above
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ++ks)
                                 umma_f16_ts(d, ka + part * C::T_LO + 8 * ks, qd + (uint64_t)((ks >> 2) * (C::Q_SUB >> 4) + 2 * (ks & 3)),
-                                            id, part > 0 || ks > 0);
+                                            id, part == 0 || ks > 0);
                         umma_commit(&bars[B_DF + b]);
                         if (b) ++filled[1]; else ++filled[0];
                     }

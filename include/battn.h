@@ -413,8 +413,8 @@ int battn_attend_sinks_paged(battn_handle* h, void* out, const void* q, const ba
  *            included.  A call that meets more sets BATTN_DEV_WORKSPACE and writes nothing.
  * The weights divide by a denominator that is summed in fp32 from unrounded weights (the output divides by the sum of the
  * fp16 weights its product uses); fp32 queries are rounded to fp16 first, as everywhere.  Measured distance of the scores from 64
- * bits (2-norm, fp16 queries): one row 2e-7 to 4e-7; a chunk, whose scores are formed on the tensor core, 1e-6 to 3e-6 at
- * head_dim 128 and 3e-6 to 6e-6 at 256.  No atomics: results repeat. */
+ * bits (2-norm, fp16 queries): one row 2e-7 to 4e-7; a chunk, whose scores are formed on the tensor core, 3e-7 to
+ * 1.3e-6.  No atomics: results repeat. */
 int battn_track_workspace_bytes(const battn_handle* h, int n_seq, int rows_per_seq, long long max_positions, size_t* out_bytes);
 int battn_attend_track(battn_handle* h, void* out, float* score_out, const float* score_in, const void* q, const uint8_t* kvk,
                        const uint8_t* kvv, const int* pos, const int* kslot, const int* act, void* ws, size_t ws_bytes, int rows,
