@@ -133,7 +133,10 @@ __device__ __forceinline__ void descend(uint32_t* hist, int C, int rank, uint32_
 }
 
 // SEL_THREADS: 1024 for few clusters, where a pass over the keys is the time; 512 once they outnumber the SMs, so that three
-// CTAs share one (32 sequences of up to 8192: 20 -> 14 us)
+// CTAs share one (32 sequences of up to 8192: 20 -> 14 us).  That holds where a partition has room for 11,000 positions or fewer: the
+// host sizes the keys by the partition, up to 160 KB, and from about 21,000 positions on one CTA of 512 has the SM to itself
+// (the whole call on 32 sequences of up to 8192 moved elsewhere: 81 us in partitions of 8192, 87 of 32768, 89 of 131072; in
+// place 72, 78, 79).
 template <int SEL_THREADS>
 __global__ void __launch_bounds__(SEL_THREADS, 1024 / SEL_THREADS) k_evict_select(const Params P) {
     extern __shared__ __align__(16) uint32_t s_key[];            // P.keys keys of this CTA's share
@@ -290,7 +293,8 @@ __device__ __forceinline__ void copy4_async(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-// Sources are 8-byte aligned only (a record is 136 or 272 bytes), targets are one run of 16-byte pieces per round and page.
+// Sources are fetched in pieces of 8 bytes: a record of 136 bytes starts on 8, one of 272 (head_dim 256) would allow 16.
+// Targets are one run of 16-byte pieces per round and page.
 template <int HD>
 __global__ void __launch_bounds__(MOVE_THREADS) k_evict_move(const Params P) {
     using C = MoveCfg<HD>;

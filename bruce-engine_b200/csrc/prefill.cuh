@@ -90,8 +90,8 @@ struct Params {
     float2* norm = nullptr;
 };
 // the partition (or table row) of a variant's sequence; -1: idle, -2: bad, nothing to do.  (Without a branch: the caller's
-// early return has to be uniform for the compiler too, or it gives up its uniform registers and spills: 626 -> 598 us for the
-// weight-accumulating call at 512 rows and 32K, 66 -> 61 us for a window chunk with sinks.)
+// early return has to be uniform for the compiler too, or it gives up its uniform registers and spills: with a branch here the
+// weight-accumulating call at 512 rows and 32K took 4 % longer, a window chunk with sinks 8 %.)
 template <int VAR>
 __device__ __forceinline__ int chunk_slot(const Params& P) {
     if (VAR == VAR_PLAIN) return P.slot;

@@ -44,9 +44,9 @@
 // chosen so that every shared-memory access of the dequant warps is bank-conflict free.
 // Every wait is bounded; a wait that runs out sets the device status word, the remaining waits are
 // skipped, tensor memory is released and the kernel returns.
-// Variants (template parameter VAR, see common.cuh): VAR_SINK walks the sink tiles before the window's; VAR_TRACK also sums the
-// unrounded weights per row (one packed add per two exponentials; 512 rows at 32K: 383 us, plain 359) for the accumulation in
-// track.cuh.
+// Variants (template parameter VAR, see common.cuh): VAR_SINK walks the sink tiles before the window's (512 rows at 16384: 66 us,
+// the plain window kernel 64); VAR_TRACK also sums the unrounded weights per row, one packed add per two exponentials, for the
+// accumulation in track.cuh (512 rows at 32K, a dozen calls in a row: 371 us, like the plain kernel).
 #pragma once
 #include "prefill.cuh"
 
